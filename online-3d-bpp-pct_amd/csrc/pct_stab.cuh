@@ -544,11 +544,10 @@ PCT_SD bool stab_split(const Geo& geo, const double bg[9], int k, const Sup& sup
       double t0 = e00 - e10, t1 = e01 - e11;
       const StabDot2 dot2{gelsd_avx2};  // (the lever rule's np.dot / np.linalg.norm follow the host flavour too)
       double len = sqrt(dot2(t0, t1, t0, t1));
-      // tri_base_len ** 2: NumPy calls libm pow(len, 2.0), which is not correctly rounded -- pct_pow.cuh restates glibc's
-      // pow as its FMA build executes it.  Geo::kSquareIsPow: every length this env can produce -- sqrt of a sum of two squares
+      // tri_base_len ** 2 (pct_pow.cuh).  Geo::kSquareIsPow: every length this env can produce -- sqrt of a sum of two squares
       // of half-integers below 32 (the 5-bit-coordinate discrete kernels) -- has pow(len, 2.0) == len * len (exhaustive up
       // to 43 per axis, tests/test_stab_host.py; the first length that differs is that of (39.5, 43.5))
-      double l2 = Geo::kSquareIsPow ? len * len : pow_glibc_fma(len, 2.0);
+      double l2 = Geo::kSquareIsPow ? len * len : lever_square(len);
       t0 /= l2; t1 /= l2;
       sp.f[0] = fabs(dot2(stk[0] - e10, stk[1] - e11, t0, t1));
       sp.f[1] = fabs(dot2(stk[0] - e00, stk[1] - e01, t0, t1));
