@@ -39,7 +39,26 @@ def _hipcc():
 def _tu_inputs(src):
     # what a translation unit is compiled from: a change elsewhere does not recompile it
     return [os.path.join(CSRC, src)] + sorted(_includes(os.path.join(CSRC, src))) + [
-        os.path.join(HERE, "..", "include", "pct_env.h"), os.path.abspath(__file__)]  # (this file holds the flags)
+        os.path.join(HERE, "..", "include", "pct_env.h")]
+
+
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
+         # the continuous env mirrors the reference's float64 operation order: no FMA contraction
+         "-ffp-contract=off",
+         # no packed float32 instructions: some of their forms have returned wrong values now and then
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+         # no real calls inside a kernel: every device function is inlined (profiles/r03_fault_root_cause.txt: this
+         # hipcc mis-places AGPR split copies around a call under a narrowed exec mask); scripts/check_no_calls.py
+         # verifies the built library
+         "-mllvm", "-amdgpu-function-calls=false", "-Wno-pass-failed"]
+
+
+def _flags_changed(src):
+    """an object remembers the flags it was compiled with in a file beside it"""
+    try:
+        return open(_obj(src) + ".flags").read() != " ".join(FLAGS)
+    except OSError:
+        return True
 
 
 def _obj(src):
@@ -55,7 +74,8 @@ def needs_build():
     # a source edited while a build was running is older than the library that build linked, but newer than the object
     # it was compiled into (objects stay in the build container; where there are none the library's own time decides)
     for src in SOURCES:
-        if os.path.exists(_obj(src)) and any(os.path.getmtime(d) > os.path.getmtime(_obj(src)) for d in _tu_inputs(src)):
+        if os.path.exists(_obj(src)) and (_flags_changed(src) or any(
+                os.path.getmtime(d) > os.path.getmtime(_obj(src)) for d in _tu_inputs(src))):
             return True
     return False
 
@@ -65,26 +85,20 @@ def build_library(force=False, verbose=False):
         return LIB
     # one hipcc per translation unit, in parallel, then a link step
     from concurrent.futures import ThreadPoolExecutor
-    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
-             # the continuous env mirrors the reference's float64 operation order: no FMA contraction
-             "-ffp-contract=off",
-             # no real calls inside a kernel: every device function is inlined (profiles/r03_fault_root_cause.txt: this
-             # hipcc mis-places AGPR split copies around a call under a narrowed exec mask); scripts/check_no_calls.py
-             # verifies the built library
-             "-mllvm", "-amdgpu-function-calls=false"]
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
 
     def compile_one(src):
         obj = _obj(src)
         srcs = _tu_inputs(src)
-        if not force and os.path.exists(obj) and all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in srcs):
+        if not force and os.path.exists(obj) and not _flags_changed(src) and all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in srcs):
             return obj
-        cmd = [_hipcc(), *flags, "-Wno-pass-failed", "-c", os.path.join(CSRC, src), "-o", obj]
+        cmd = [_hipcc(), *FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd))
         t0 = time.time()
         subprocess.check_call(cmd)
+        open(obj + ".flags", "w").write(" ".join(FLAGS))
         if verbose:
             print("%s: %.0f s" % (src, time.time() - t0))
         return obj
