@@ -14,7 +14,8 @@ LIB = os.path.join(HERE, "libpct_hip.so")
 # (slowest translation units first: they are handed to the worker pool in this order)
 SOURCES = ["pct_discrete_stab.hip", "pct_discrete_stab_mt.hip", "pct_discrete_u64_stab.hip", "pct_discrete_u64_stab_mt.hip",
            "pct_continuous.hip", "pct_continuous_mt.hip", "pct_continuous_pipe.hip", "pct_discrete.hip", "pct_discrete_mt.hip", "pct_discrete_u64.hip",
-           "pct_discrete_u64_mt.hip", "pct_env.hip"]
+           "pct_discrete_u64_mt.hip", "pct_env.hip", "pct_choice.hip", "pct_attend.hip", "pct_attend_f32.hip",
+           "pct_attend_bf16.hip", "pct_attend_f16.hip"]
 
 
 def _includes(path, seen=None):
@@ -39,7 +40,8 @@ def _hipcc():
 def _tu_inputs(src):
     # what a translation unit is compiled from: a change elsewhere does not recompile it
     return [os.path.join(CSRC, src)] + sorted(_includes(os.path.join(CSRC, src))) + [
-        os.path.join(HERE, "..", "include", "pct_env.h")]
+        os.path.join(HERE, "..", "include", h) for h in ("pct_env.h", "pct_policy.h")
+        if h == "pct_env.h" or src.startswith(("pct_choice", "pct_attend"))]
 
 
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

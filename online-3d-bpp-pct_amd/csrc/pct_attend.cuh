@@ -1,0 +1,776 @@
+// pct_attend.cuh -- attention of the queries of a batch to its allowed keys, and the gradients.
+//
+// For the rows r = (l, g) of one key/value head (g counts the heads that share it), over the n allowed keys j of the batch:
+//     S_rj = q_r . k_j,  P_rj = e^(scale S_rj) / sum_j e^(scale S_rj),  O_r = sum_j P_rj v_j   (n = 0: O = 0, no gradients)
+//     D_r = dO_r . O_r = sum_j P_rj dP_rj,  dP_rj = dO_r . v_j,  dS_rj = P_rj (dP_rj - D_r),
+//     dq_r = scale sum_j dS_rj k_j,   dk_j = scale sum_r dS_rj q_r,   dv_j = sum_r P_rj dO_r.
+//
+// A mask allows a key for every query of its batch, so the allowed keys are listed once (pct_attend_list_kernel) and only they
+// are read: the work falls with their share, nothing masked is multiplied, and a value that must not count is never loaded.
+//
+// One layout carries the three kernels.  A wavefront keeps 32 "resident" rows, one to a lane column (rows of q in the forward
+// and the dq kernel, keys in the dk/dv kernel), and walks over tiles of "streamed" rows that the workgroup stages in LDS.  With
+// 32x32x16 matrix instructions a product streamed x resident^T leaves in lane (c, h) = (lane % 32, lane / 32) column c and the
+// rows {8 i + 4 h .. + 3}.  The second product contracts over these rows, and the order of a contraction is free as long as
+// both operands share it: registers 8 b .. 8 b + 7 of the lane ARE its operand for the block of 16 rows b, where slot (h, e)
+// means row 16 b + 8 (e / 4) + 4 h + e % 4.  So P and dS never pass through LDS or another lane; the other operand is read from
+// the staged tile transposed (ds_read_b64_tr_b16), in that row order.  The sum of a row and its maximum are a lane's own
+// registers and one exchange between the halves.
+//
+// float32 runs the same code with eight 32x32x2 instructions in place of one 32x32x16 (slot e of both halves each).
+//
+// Roundings: S, P, dP, dS, all sums and statistics are float32.  P and dS are rounded to the tensors' type as operands of the
+// second product (half a step, as the result itself is); float32 tensors stay float32.  In float16, whose range is small, P
+// carries a power of two, and dS one that follows the largest entry met so far (pct_attend: F16 below).
+#ifndef PCT_ATTEND_CUH
+#define PCT_ATTEND_CUH
+#include <type_traits>
+
+#include "pct_policy.cuh"
+
+namespace pct {
+
+struct AttendParams {
+  const void *q, *k, *v, *d_out, *o;
+  int64_t qs[3], ks[3], vs[3], ds[3];  // batch, length, head
+  const int32_t* list;                 // [batch, k_len + 1]: the count, the allowed keys, then the others
+  const void* lengths;
+  int lengths_type;
+  int batch, q_len, k_len, heads, kv_heads, dim, group, rows;  // rows = q_len * group
+  float scale, c;                      // c = scale log2 e
+  int tiles, splits;                   // workgroups along the resident rows / along the streamed ones
+  void* out;
+  float2* stats;                       // [batch, kv_heads, rows]: reference point (log2), sum
+  float* delta;                        // [batch, kv_heads, rows]
+  void *dq, *dk, *dv;
+  float* part;                         // splits > 1: float32 partial results
+  float2* part_stats;
+};
+
+namespace {
+
+template <typename T> using Frag = T __attribute__((ext_vector_type(8)));
+typedef float Acc __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ Acc mfma(Frag<bf16> a, Frag<bf16> b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ Acc mfma(Frag<f16> a, Frag<f16> b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ Acc mfma(Frag<float> a, Frag<float> b, Acc c) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+template <typename T> struct Type {
+  static constexpr int CE = 16 / sizeof(T);           // elements to a 16-byte chunk
+  static constexpr int ROWS = sizeof(T) == 2 ? 64 : 32;  // streamed rows to a tile
+  static constexpr bool F16 = __is_same(T, f16);
+};
+
+#define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
+
+// a staged tile: rows of DP elements in 16-byte chunks; a chunk's place within its row is XORed with bits of the row so that 16
+// adjacent rows at one chunk, and 4 adjacent rows at two, meet different banks
+template <typename T, int DP>
+struct Tile {
+  static constexpr int CE = Type<T>::CE, CPR = DP / CE, ROWS = Type<T>::ROWS, BYTES = ROWS * DP * (int)sizeof(T);
+  static __device__ __forceinline__ int swz(int row) { return CPR % 16 == 0 ? row & 15 : (CPR % 8 == 0 ? (row >> 1) & 7 : (row >> 2) & 3); }
+  static __device__ __forceinline__ int at(int row, int d) { return row * DP + ((d / CE) ^ swz(row)) * CE + d % CE; }
+
+  // 8 elements along d: the first product's operand
+  static __device__ __forceinline__ Frag<T> row8(const T* t, int row, int d) {
+    if constexpr (sizeof(T) == 2) {
+      return *(const Frag<T>*)(t + at(row, d));
+    } else {
+      typedef float f4 __attribute__((ext_vector_type(4)));
+      const f4 a = *(const f4*)(t + at(row, d)), b = *(const f4*)(t + at(row, d + 4));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  // 8 rows of column d0 + lane % 32, in the order of the second product's slots: rows r0 + 4 h + {0..3, 8..11}
+  static __device__ __forceinline__ Frag<T> col8(const T* t, int r0, int d0, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      const int i = lane & 15, row = r0 + 4 * h + (i >> 2), d = d0 + (lane & 16) + 4 * (i & 3);
+      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s4, (T*)t + at(row, d)));
+      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s4, (T*)t + at(row + 8, d)));
+      return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      Frag<T> f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[e] = t[at(r0 + 8 * (e >> 2) + 4 * h + (e & 3), d0 + (lane & 31))];
+      return f;
+    }
+  }
+  // starts the copy of the tile's rows from global memory straight into LDS, 64 chunks to an instruction; the caller waits.
+  // What lies behind `dim` in a row is left as it is (zero from the start).
+  template <typename Row>
+  static __device__ __forceinline__ void stage(T* t, int dim, int wave, int waves, int lane, Row row_ptr) {
+    for (int i = wave; i < ROWS * CPR / 64; i += waves) {
+      const int c = i * 64 + lane, row = c / CPR, d = ((c % CPR) ^ swz(row)) * CE;
+      const T* src = row_ptr(row) + d;
+      if (d < dim)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, LDS_PTR(void, t + i * 64 * CE), 16, 0, 0);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ Frag<T> load_frag(const T* p) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw { T v[8]; };
+  const Raw r = *(const Raw*)p;
+  return __builtin_bit_cast(Frag<T>, r);
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> zero_frag() {
+  Frag<T> f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) f[e] = (T)0.f;
+  return f;
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> to_frag(const float* v) {
+  if constexpr (sizeof(T) == 4) {
+    Frag<T> f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = v[e];
+    return f;
+  } else {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const u4 w = {pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])};
+    return __builtin_bit_cast(Frag<T>, w);
+  }
+}
+// 4 adjacent elements of an output row
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 4) {
+    *(float4*)p = make_float4(a, b, c, d);
+  } else {
+    *(uint2*)p = make_uint2(pack2<T>(a, b), pack2<T>(c, d));
+  }
+}
+__device__ __forceinline__ float other_half(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ int allowed_keys(const AttendParams& p, int b) {
+  if (p.list) return p.list[(int64_t)b * (p.k_len + 1)];
+  if (!p.lengths) return p.k_len;
+  const int64_t n = p.lengths_type == 8 ? ((const int64_t*)p.lengths)[b] : ((const int32_t*)p.lengths)[b];
+  return (int)(n < 0 ? 0 : (n > p.k_len ? p.k_len : n));
+}
+
+// the row of register j of an accumulator
+__device__ __forceinline__ int acc_row(int j, int h) { return (j & 3) + 8 * (j >> 2) + 4 * h; }
+
+struct Work { int b, kh, tile, split; };
+// Workgroups go to the 8 dies in turn, and each die has an L2 of its own: the workgroups that stream the same rows are numbered
+// so that they meet on one die.
+__device__ __forceinline__ Work decode(const AttendParams& p) {
+  const int total = gridDim.x, die = blockIdx.x & 7, slot = blockIdx.x >> 3, per = total >> 3, rest = total & 7;
+  int w = die * per + (die < rest ? die : rest) + slot;
+  Work k;
+  k.tile = w % p.tiles; w /= p.tiles;
+  k.split = w % p.splits; w /= p.splits;
+  k.kh = w % p.kv_heads;
+  k.b = w / p.kv_heads;
+  return k;
+}
+
+// element offset of row r = (l, g) of a [batch, length, head, dim] tensor
+__device__ __forceinline__ int64_t row_offset(const int64_t (&s)[3], const AttendParams& p, int b, int kh, int r) {
+  const int l = p.group == 1 ? r : r / p.group, g = r - l * p.group;
+  return b * s[0] + l * s[1] + (int64_t)(kh * p.group + g) * s[2];
+}
+__device__ __forceinline__ int64_t out_offset(const AttendParams& p, int b, int kh, int r) {
+  const int l = p.group == 1 ? r : r / p.group, g = r - l * p.group;
+  return (((int64_t)b * p.q_len + l) * p.heads + kh * p.group + g) * p.dim;
+}
+
+template <int N>
+__device__ __forceinline__ void zero_lds(void* p, int tid, int threads) {
+  for (int i = tid; i < N / 16; i += threads) ((float4*)p)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// the staged tile is there, the other one is free: every wavefront waits for its own copies, then for the others
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// F16: the power of two that dS carries into its product, one for the wavefront.  It starts high and falls so that the largest
+// entry met so far stays below 2^14; when it falls, the sums so far are scaled with it.
+struct Power {
+  int e;
+  __device__ __forceinline__ void start() { e = 100; }
+  template <int N>
+  __device__ __forceinline__ float follow(float largest, Acc (&acc)[N]) {
+    const float m = wave_max(largest);
+    const int x = (int)((__float_as_uint(m) >> 23) & 255) - 127;  // 2^x <= m < 2^(x + 1)
+    int want = 13 - x;
+    want = want < -100 ? -100 : want;
+    if (m > 0.f && want < e) {
+      const float f = __builtin_amdgcn_exp2f((float)(want - e));
+#pragma unroll
+      for (int i = 0; i < N; i++) acc[i] *= f;
+      e = want;
+    }
+    return __builtin_amdgcn_exp2f((float)e);
+  }
+};
+
+// ------------------------------------------------------------------------------------------------------------- forward
+template <typename T, int DP, int MAXW>
+__global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
+  using L = Tile<T, DP>;
+  constexpr int KT = L::ROWS, SUB = KT / 32, KS = DP / 16, DB = DP / 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* const buf = (T*)lds;  // [2][k, v] tiles
+  __shared__ int keys[2][KT];
+  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6, c32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Work w = decode(p);
+  const int n = allowed_keys(p, w.b), all = (n + KT - 1) / KT;
+  const int t0 = (int)((int64_t)all * w.split / p.splits), t1 = (int)((int64_t)all * (w.split + 1) / p.splits);
+  const int row = (w.tile * waves + wave) * 32 + c32;
+  const bool active = (w.tile * waves + wave) * 32 < p.rows;
+  const int32_t* list = p.list ? p.list + (int64_t)w.b * (p.k_len + 1) + 1 : nullptr;
+  const T* kb = (const T*)p.k + w.b * p.ks[0] + w.kh * p.ks[2];
+  const T* vb = (const T*)p.v + w.b * p.vs[0] + w.kh * p.vs[2];
+
+  auto key_at = [&](int i) { i = i < n ? i : n - 1; return list ? list[i] : i; };
+  auto stage = [&](int t) {
+    T* k = buf + (t & 1) * 2 * KT * DP;
+    L::stage(k, p.dim, wave, waves, lane, [&](int r) { return kb + keys[t & 1][r] * p.ks[1]; });
+    L::stage(k + KT * DP, p.dim, wave, waves, lane, [&](int r) { return vb + keys[t & 1][r] * p.vs[1]; });
+  };
+  if (p.dim != DP) zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
+  if (t0 < t1) {
+    for (int i = tid; i < KT; i += blockDim.x) {
+      keys[t0 & 1][i] = key_at(t0 * KT + i);
+      keys[(t0 + 1) & 1][i] = key_at((t0 + 1) * KT + i);
+    }
+  }
+  Frag<T> qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; s++) {
+    const int d = 16 * s + 8 * h;
+    qf[s] = row < p.rows && d < p.dim ? load_frag((const T*)p.q + row_offset(p.qs, p, w.b, w.kh, row) + d) : zero_frag<T>();
+  }
+  __syncthreads();
+  if (t0 < t1) stage(t0);
+  Acc o[DB];
+#pragma unroll
+  for (int i = 0; i < DB; i++) o[i] = Acc{};
+  // exponents are taken against `ref`, which follows the maximum only when it is left behind by more than 2^6 (P then stays
+  // small enough for every type, and the sums are rarely scaled); float16 lifts P by 2^8 out of its denormals
+  constexpr float LIFT = Type<T>::F16 ? 8.f : 0.f;
+  float ref = -INFINITY, sum = 0.f;
+  for (int t = t0; t < t1; t++) {
+    tile_barrier();
+    int ahead = 0;
+    if (t + 1 < t1) stage(t + 1);
+    if (t + 2 < t1 && tid < KT) ahead = key_at((t + 2) * KT + tid);
+    if (active) {
+      const T* kt = buf + (t & 1) * 2 * KT * DP;
+      const T* vt = kt + KT * DP;
+      Acc s[SUB];
+#pragma unroll
+      for (int i = 0; i < SUB; i++) {
+        s[i] = Acc{};
+#pragma unroll
+        for (int x = 0; x < KS; x++) s[i] = mfma(L::row8(kt, 32 * i + c32, 16 * x + 8 * h), qf[x], s[i]);
+      }
+      if ((t + 1) * KT > n) {
+#pragma unroll
+        for (int i = 0; i < SUB; i++)
+#pragma unroll
+          for (int j = 0; j < 16; j++) s[i][j] = t * KT + 32 * i + acc_row(j, h) < n ? s[i][j] : -INFINITY;
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) top = fmaxf(top, s[i][j]);
+      top = fmaxf(top, other_half(top)) * p.c - LIFT;
+      if (__ballot(top > ref + 6.f)) {
+        const float to = fmaxf(ref, top), f = __builtin_amdgcn_exp2f(ref - to);
+#pragma unroll
+        for (int i = 0; i < DB; i++) o[i] *= f;
+        sum *= f;
+        ref = to;
+      }
+#pragma unroll
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          s[i][j] = __builtin_amdgcn_exp2f(fmaf(s[i][j], p.c, -ref));
+          sum += s[i][j];
+        }
+#pragma unroll
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          float e8[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) e8[e] = s[i][8 * b + e];
+          const Frag<T> pf = to_frag<T>(e8);
+#pragma unroll
+          for (int d = 0; d < DB; d++) o[d] = mfma(L::col8(vt, 32 * i + 16 * b, 32 * d, lane), pf, o[d]);
+        }
+    }
+    if (t + 2 < t1) {  // (every wavefront has read the keys of tile t before the barrier above)
+      if (tid < KT) keys[t & 1][tid] = ahead;
+      for (int i = tid + (int)blockDim.x; i < KT; i += blockDim.x) keys[t & 1][i] = key_at((t + 2) * KT + i);
+    }
+  }
+  if (row >= p.rows) return;
+  sum += other_half(sum);
+  const int64_t at = ((int64_t)w.b * p.kv_heads + w.kh) * p.rows + row;
+  if (p.splits > 1) {
+    const int64_t sp = (int64_t)w.split * p.batch * p.kv_heads * p.rows + at;
+    if (h == 0) p.part_stats[sp] = make_float2(ref, sum);
+    float* dst = p.part + sp * p.dim;
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int d = 32 * i + 8 * j + 4 * h;
+        if (d < p.dim) *(float4*)(dst + d) = make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
+      }
+    return;
+  }
+  const float inv = n > 0 ? 1.f / sum : 0.f;
+  if (h == 0 && p.stats) p.stats[at] = n > 0 ? make_float2(ref, sum) : make_float2(0.f, INFINITY);
+  T* dst = (T*)p.out + out_offset(p, w.b, w.kh, row);
+#pragma unroll
+  for (int i = 0; i < DB; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int d = 32 * i + 8 * j + 4 * h;
+      if (d < p.dim) store4<T>(dst + d, o[i][4 * j] * inv, o[i][4 * j + 1] * inv, o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv);
+    }
+}
+
+// joins the splits of the forward pass: a thread to 4 elements of a row
+template <typename T>
+__global__ __launch_bounds__(256) void pct_attend_join_kernel(AttendParams p) {
+  const int per = p.dim / 4;
+  const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * per) return;
+  const int64_t at = i / per;
+  const int d = (int)(i % per) * 4, r = (int)(at % p.rows), bh = (int)(at / p.rows);
+  float ref = -INFINITY, sum = 0.f;
+  for (int s = 0; s < p.splits; s++) ref = fmaxf(ref, p.part_stats[s * rows + at].x);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (ref > -INFINITY)
+    for (int s = 0; s < p.splits; s++) {
+      const float2 st = p.part_stats[s * rows + at];
+      const float f = __builtin_amdgcn_exp2f(st.x - ref);
+      const float4 x = *(const float4*)(p.part + (s * rows + at) * p.dim + d);
+      sum += f * st.y;
+      o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
+    }
+  const bool none = allowed_keys(p, bh / p.kv_heads) == 0;
+  const float inv = none ? 0.f : 1.f / sum;
+  if (d == 0 && p.stats) p.stats[at] = none ? make_float2(0.f, INFINITY) : make_float2(ref, sum);
+  store4<T>((T*)p.out + out_offset(p, bh / p.kv_heads, bh % p.kv_heads, r) + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// P of the backward pass: float32 keeps the forward's reference point and sum apart (their logarithm's rounding would be a
+// common factor of the row), the others fold them, and float16 lifts P by 2^14 (P <= 1)
+template <typename T> constexpr float p_lift() { return Type<T>::F16 ? 14.f : 0.f; }
+template <typename T>
+__device__ __forceinline__ float2 p_terms(float2 st) {
+  if constexpr (sizeof(T) == 4) return make_float2(st.x, 1.f / st.y);
+  else return make_float2(st.x + log2f(st.y) - p_lift<T>(), 1.f);
+}
+template <typename T>
+__device__ __forceinline__ float p_value(float s, float c, float2 t) {
+  const float e = __builtin_amdgcn_exp2f(fmaf(s, c, -t.x));
+  return sizeof(T) == 4 ? e * t.y : e;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- dq, D
+// D_r = dO_r . O_r, where O_r has been rounded to the tensors' type: over many keys that error vanishes beside dP, over few it
+// would not, so where all keys fit one tile D is summed from P dP itself.
+template <typename T, int DP, int MAXW>
+__global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p) {
+  using L = Tile<T, DP>;
+  constexpr int KT = L::ROWS, SUB = KT / 32, KS = DP / 16, DB = DP / 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* const buf = (T*)lds;
+  __shared__ int keys[2][KT];
+  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6, c32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Work w = decode(p);
+  const int n = allowed_keys(p, w.b), all = (n + KT - 1) / KT;
+  const int t0 = (int)((int64_t)all * w.split / p.splits), t1 = (int)((int64_t)all * (w.split + 1) / p.splits);
+  const int row = (w.tile * waves + wave) * 32 + c32;
+  const bool active = (w.tile * waves + wave) * 32 < p.rows;
+  const int32_t* list = p.list ? p.list + (int64_t)w.b * (p.k_len + 1) + 1 : nullptr;
+  const T* kb = (const T*)p.k + w.b * p.ks[0] + w.kh * p.ks[2];
+  const T* vb = (const T*)p.v + w.b * p.vs[0] + w.kh * p.vs[2];
+  const int64_t at = ((int64_t)w.b * p.kv_heads + w.kh) * p.rows + row;
+
+  auto key_at = [&](int i) { i = i < n ? i : n - 1; return list ? list[i] : i; };
+  auto stage = [&](int t) {
+    T* k = buf + (t & 1) * 2 * KT * DP;
+    L::stage(k, p.dim, wave, waves, lane, [&](int r) { return kb + keys[t & 1][r] * p.ks[1]; });
+    L::stage(k + KT * DP, p.dim, wave, waves, lane, [&](int r) { return vb + keys[t & 1][r] * p.vs[1]; });
+  };
+  if (p.dim != DP) zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
+  if (t0 < t1) {
+    for (int i = tid; i < KT; i += blockDim.x) {
+      keys[t0 & 1][i] = key_at(t0 * KT + i);
+      keys[(t0 + 1) & 1][i] = key_at((t0 + 1) * KT + i);
+    }
+  }
+  Frag<T> qf[KS], df[KS];
+  float D = 0.f;
+  float2 st = make_float2(INFINITY, 0.f);
+  if (row < p.rows && n > 0) st = p_terms<T>(p.stats[at]);
+#pragma unroll
+  for (int s = 0; s < KS; s++) {
+    const int d = 16 * s + 8 * h;
+    const bool in = row < p.rows && d < p.dim;
+    qf[s] = in ? load_frag((const T*)p.q + row_offset(p.qs, p, w.b, w.kh, row) + d) : zero_frag<T>();
+    df[s] = in ? load_frag((const T*)p.d_out + row_offset(p.ds, p, w.b, w.kh, row) + d) : zero_frag<T>();
+    if (in && n > KT) {
+      const Frag<T> of = load_frag((const T*)p.o + out_offset(p, w.b, w.kh, row) + d);
+#pragma unroll
+      for (int e = 0; e < 8; e++) D = fmaf((float)df[s][e], (float)of[e], D);
+    }
+  }
+  __syncthreads();
+  if (t0 < t1) stage(t0);
+  Acc dq[DB];
+#pragma unroll
+  for (int i = 0; i < DB; i++) dq[i] = Acc{};
+  Power power;
+  power.start();
+  auto products = [&](const T* kt, const T* vt, int first, Acc& s, Acc& dp) {  // P in s, dP in dp, of 32 keys
+    s = Acc{};
+    dp = Acc{};
+#pragma unroll
+    for (int x = 0; x < KS; x++) {
+      s = mfma(L::row8(kt, first % KT + c32, 16 * x + 8 * h), qf[x], s);
+      dp = mfma(L::row8(vt, first % KT + c32, 16 * x + 8 * h), df[x], dp);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++) s[j] = first + acc_row(j, h) < n ? p_value<T>(s[j], p.c, st) : 0.f;
+  };
+  for (int t = t0; t < t1; t++) {
+    tile_barrier();
+    int ahead = 0;
+    if (t + 1 < t1) stage(t + 1);
+    if (t + 2 < t1 && tid < KT) ahead = key_at((t + 2) * KT + tid);
+    if (active) {
+      const T* kt = buf + (t & 1) * 2 * KT * DP;
+      const T* vt = kt + KT * DP;
+      if (n <= KT) {
+#pragma unroll 1
+        for (int i = 0; i < SUB; i++) {
+          Acc s, dp;
+          products(kt, vt, 32 * i, s, dp);
+#pragma unroll
+          for (int j = 0; j < 16; j++) D = fmaf(s[j], dp[j], D);
+        }
+        D *= __builtin_amdgcn_exp2f(-p_lift<T>());
+      }
+      if (t == t0) D += other_half(D);
+#pragma unroll 1
+      for (int i = 0; i < SUB; i++) {
+        if (t * KT + 32 * i >= n) break;
+        Acc s, dp;
+        products(kt, vt, t * KT + 32 * i, s, dp);
+        float e16[16], big = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          e16[j] = s[j] * (dp[j] - D);
+          if (Type<T>::F16) big = fmaxf(big, fabsf(e16[j]));
+        }
+        if (Type<T>::F16) {
+          const float f = power.follow(big, dq);
+#pragma unroll
+          for (int j = 0; j < 16; j++) e16[j] *= f;
+        }
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const Frag<T> sf = to_frag<T>(e16 + 8 * b);
+#pragma unroll
+          for (int d = 0; d < DB; d++) dq[d] = mfma(L::col8(kt, 32 * i + 16 * b, 32 * d, lane), sf, dq[d]);
+        }
+      }
+    }
+    if (t + 2 < t1) {  // (every wavefront has read the keys of tile t before the barrier above)
+      if (tid < KT) keys[t & 1][tid] = ahead;
+      for (int i = tid + (int)blockDim.x; i < KT; i += blockDim.x) keys[t & 1][i] = key_at((t + 2) * KT + i);
+    }
+  }
+  if (row >= p.rows) return;
+  if (h == 0 && t0 == 0 && t1 > 0) p.delta[at] = D;  // (one split of them has the first tile; without keys nobody reads it)
+  const float f = Type<T>::F16 ? p.scale * __builtin_amdgcn_exp2f(-(float)power.e - p_lift<T>()) : p.scale;
+  float* part = p.splits > 1 ? p.part + (int64_t)w.split * p.batch * p.q_len * p.heads * p.dim + out_offset(p, w.b, w.kh, row) : nullptr;
+  T* dst = (T*)p.dq + out_offset(p, w.b, w.kh, row);
+#pragma unroll
+  for (int i = 0; i < DB; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int d = 32 * i + 8 * j + 4 * h;
+      if (d >= p.dim) continue;
+      const float a = dq[i][4 * j] * f, b = dq[i][4 * j + 1] * f, c = dq[i][4 * j + 2] * f, e = dq[i][4 * j + 3] * f;
+      if (part) *(float4*)(part + d) = make_float4(a, b, c, e);
+      else store4<T>(dst + d, a, b, c, e);
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------------- dk, dv
+template <typename T, int DP, int MAXW>
+__global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams p) {
+  using L = Tile<T, DP>;
+  constexpr int QT = L::ROWS, SUB = QT / 32, KS = DP / 16, DB = DP / 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* const buf = (T*)lds;  // [2][q, d_out] tiles
+  __shared__ __attribute__((aligned(16))) float terms[2][3][QT];  // of the staged rows: p_terms, D
+  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6, c32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Work w = decode(p);
+  const int n = allowed_keys(p, w.b);
+  const int first = (w.tile * waves + wave) * 32, i = first + c32;  // place in the list
+  const bool active = first < n, valid = i < n;
+  const bool any = w.tile * waves * 32 < n;  // (of the workgroup)
+  const int all = any ? (p.rows + QT - 1) / QT : 0;
+  const int t0 = (int)((int64_t)all * w.split / p.splits), t1 = (int)((int64_t)all * (w.split + 1) / p.splits);
+  const int32_t* list = p.list ? p.list + (int64_t)w.b * (p.k_len + 1) + 1 : nullptr;
+  const int key = i < p.k_len ? (list ? list[i] : i) : 0;
+  const float2* stats = p.stats + ((int64_t)w.b * p.kv_heads + w.kh) * p.rows;
+  const float* delta = p.delta + ((int64_t)w.b * p.kv_heads + w.kh) * p.rows;
+
+  auto stage = [&](int t) {
+    T* q = buf + (t & 1) * 2 * QT * DP;
+    auto at = [&](int r) { r += t * QT; return r < p.rows ? r : p.rows - 1; };
+    L::stage(q, p.dim, wave, waves, lane, [&](int r) { return (const T*)p.q + row_offset(p.qs, p, w.b, w.kh, at(r)); });
+    L::stage(q + QT * DP, p.dim, wave, waves, lane, [&](int r) { return (const T*)p.d_out + row_offset(p.ds, p, w.b, w.kh, at(r)); });
+  };
+  auto put_terms = [&](int t) {
+    for (int r = tid; r < QT; r += blockDim.x) {
+      const int row = t * QT + r;
+      const float2 x = row < p.rows ? p_terms<T>(stats[row]) : make_float2(INFINITY, 0.f);
+      terms[t & 1][0][r] = x.x;
+      terms[t & 1][1][r] = x.y;
+      terms[t & 1][2][r] = row < p.rows ? delta[row] : 0.f;
+    }
+  };
+  if (p.dim != DP) zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
+  Frag<T> kf[KS], vf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; s++) {
+    const int d = 16 * s + 8 * h;
+    const bool in = valid && d < p.dim;
+    kf[s] = in ? load_frag((const T*)p.k + w.b * p.ks[0] + key * p.ks[1] + w.kh * p.ks[2] + d) : zero_frag<T>();
+    vf[s] = in ? load_frag((const T*)p.v + w.b * p.vs[0] + key * p.vs[1] + w.kh * p.vs[2] + d) : zero_frag<T>();
+  }
+  __syncthreads();
+  if (t0 < t1) { stage(t0); put_terms(t0); }
+  Acc dk[DB], dv[DB];
+#pragma unroll
+  for (int d = 0; d < DB; d++) { dk[d] = Acc{}; dv[d] = Acc{}; }
+  Power power;
+  power.start();
+  for (int t = t0; t < t1; t++) {
+    tile_barrier();
+    if (t + 1 < t1) { stage(t + 1); put_terms(t + 1); }
+    if (!active) continue;
+    const T* qt = buf + (t & 1) * 2 * QT * DP;
+    const T* dt = qt + QT * DP;
+#pragma unroll 1
+    for (int u = 0; u < SUB; u++) {
+      if (t * QT + 32 * u >= p.rows) break;
+      Acc s = {}, dp = {};
+#pragma unroll
+      for (int x = 0; x < KS; x++) {
+        s = mfma(L::row8(qt, 32 * u + c32, 16 * x + 8 * h), kf[x], s);
+        dp = mfma(L::row8(dt, 32 * u + c32, 16 * x + 8 * h), vf[x], dp);
+      }
+      float p16[16], e16[16], big = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int r = 32 * u + 8 * g + 4 * h;
+        const float4 a = *(const float4*)&terms[t & 1][0][r], D = *(const float4*)&terms[t & 1][2][r];
+        float4 b = make_float4(1.f, 1.f, 1.f, 1.f);
+        if (sizeof(T) == 4) b = *(const float4*)&terms[t & 1][1][r];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int j = 4 * g + e;
+          p16[j] = p_value<T>(s[j], p.c, make_float2((&a.x)[e], (&b.x)[e]));
+          e16[j] = p16[j] * (dp[j] - (&D.x)[e]);
+          if (Type<T>::F16) big = fmaxf(big, fabsf(e16[j]));
+        }
+      }
+      if (Type<T>::F16) {
+        const float f = power.follow(valid ? big : 0.f, dk);
+#pragma unroll
+        for (int j = 0; j < 16; j++) e16[j] *= f;
+      }
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const Frag<T> pf = to_frag<T>(p16 + 8 * b), sf = to_frag<T>(e16 + 8 * b);
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+          dv[d] = mfma(L::col8(dt, 32 * u + 16 * b, 32 * d, lane), pf, dv[d]);
+          dk[d] = mfma(L::col8(qt, 32 * u + 16 * b, 32 * d, lane), sf, dk[d]);
+        }
+      }
+    }
+  }
+  if (i >= p.k_len) return;
+  const float fk = Type<T>::F16 ? p.scale * __builtin_amdgcn_exp2f(-(float)power.e - p_lift<T>()) : p.scale;
+  const float fv = __builtin_amdgcn_exp2f(-p_lift<T>());
+  const int64_t at = (((int64_t)w.b * p.k_len + key) * p.kv_heads + w.kh) * p.dim;
+  const int64_t whole = (int64_t)p.batch * p.k_len * p.kv_heads * p.dim;
+  float* part = p.splits > 1 ? p.part + (int64_t)w.split * 2 * whole + at : nullptr;
+#pragma unroll
+  for (int x = 0; x < DB; x++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int d = 32 * x + 8 * j + 4 * h;
+      if (d >= p.dim) continue;
+      float k4[4], v4[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        k4[e] = valid ? dk[x][4 * j + e] * fk : 0.f;
+        v4[e] = valid ? dv[x][4 * j + e] * fv : 0.f;
+      }
+      if (part) {
+        *(float4*)(part + d) = make_float4(k4[0], k4[1], k4[2], k4[3]);
+        *(float4*)(part + whole + d) = make_float4(v4[0], v4[1], v4[2], v4[3]);
+      } else {
+        store4<T>((T*)p.dk + at + d, k4[0], k4[1], k4[2], k4[3]);
+        store4<T>((T*)p.dv + at + d, v4[0], v4[1], v4[2], v4[3]);
+      }
+    }
+}
+
+// adds the splits' partial gradients, laid out as the results are: 4 elements to a thread
+template <typename T>
+__global__ __launch_bounds__(256) void pct_attend_sum_kernel(const float* part, int64_t stride, int splits, int64_t count, T* a, T* b) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= count) return;
+  float4 s = *(const float4*)(part + blockIdx.y * count + i);
+  for (int k = 1; k < splits; k++) {
+    const float4 x = *(const float4*)(part + k * stride + blockIdx.y * count + i);
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
+  store4<T>((blockIdx.y ? b : a) + i, s.x, s.y, s.z, s.w);
+}
+
+// How the work is cut.  Resident rows: 32 to a wavefront, as many wavefronts to a workgroup as there are rows for (they share a
+// staged tile), but fewer while that leaves compute units without a workgroup.  Streamed rows: split over workgroups until
+// about four wavefronts per compute unit are there, in parts of at least two tiles; the partial results are joined after.
+struct Cut { int waves, tiles, splits; };
+inline Cut cut(int64_t resident, int64_t streamed_tiles, int64_t heads, int max_waves) {
+  const int64_t t = (resident + 31) / 32;
+  int64_t w = t < max_waves ? t : max_waves, blocks = (t + w - 1) / w;
+  w = (t + blocks - 1) / blocks;
+  while (heads * blocks < 256 && w > 1) {
+    w = (w + 1) / 2;
+    blocks = (t + w - 1) / w;
+  }
+  int64_t s = (1024 + heads * t - 1) / (heads * t);
+  s = s < streamed_tiles / 2 ? s : streamed_tiles / 2;
+  s = s < 1 ? 1 : (s > 64 ? 64 : s);
+  return Cut{(int)w, (int)blocks, (int)s};
+}
+
+// wavefronts to a workgroup: 8, two to a SIMD, where a wavefront's registers allow it (256 each)
+template <typename T, int DP> constexpr int max_waves() { return sizeof(T) == 4 && DP > 64 ? 4 : 8; }
+
+// a launch with the LDS of four tiles, which may be more than the runtime's default limit of 64 KiB
+template <int BYTES>
+void launch(void (*kernel)(AttendParams), dim3 grid, int waves, hipStream_t s, const AttendParams& p) {
+  if (BYTES > 60 * 1024) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+  kernel<<<grid, 64 * waves, BYTES, s>>>(p);
+}
+
+template <typename T> struct Attend {
+  template <typename F>
+  static auto by_dim(int dim, F f) {
+    if (dim <= 32) return f(std::integral_constant<int, 32>());
+    if (dim <= 64) return f(std::integral_constant<int, 64>());
+    if (dim <= 96) return f(std::integral_constant<int, 96>());
+    return f(std::integral_constant<int, 128>());
+  }
+  static Cut cut_q(const AttendParams& p) {
+    const int mw = by_dim(p.dim, [](auto d) { return max_waves<T, d.value>(); });
+    return cut(p.rows, (p.k_len + Type<T>::ROWS - 1) / Type<T>::ROWS, (int64_t)p.batch * p.kv_heads, mw);
+  }
+  static Cut cut_k(const AttendParams& p) {
+    const int mw = by_dim(p.dim, [](auto d) { return max_waves<T, d.value>(); });
+    return cut(p.k_len, (p.rows + Type<T>::ROWS - 1) / Type<T>::ROWS, (int64_t)p.batch * p.kv_heads, mw);
+  }
+  static int64_t workspace(const AttendParams& p, bool backward) {
+    const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows;
+    const Cut q = cut_q(p);
+    if (!backward) return q.splits > 1 ? q.splits * rows * (8 + 4 * (int64_t)p.dim) : 0;
+    const Cut k = cut_k(p);
+    const int64_t a = q.splits > 1 ? q.splits * rows * p.dim * 4 : 0;
+    const int64_t b = k.splits > 1 ? k.splits * 2 * (int64_t)p.batch * p.k_len * p.kv_heads * p.dim * 4 : 0;
+    return (rows * 4 + 255) / 256 * 256 + (a > b ? a : b);
+  }
+  static int grid(const AttendParams& p, const Cut& c, dim3& g) {
+    const int64_t n = (int64_t)c.tiles * c.splits * p.batch * p.kv_heads;
+    if (n * c.waves * 64 >= (int64_t)1 << 32) return policy_fail(PCT_ERR_UNSUPPORTED, "attention: more workgroups than a launch can hold");
+    g = dim3((unsigned)n);
+    return PCT_OK;
+  }
+  static int forward(AttendParams& p, char* ws, hipStream_t s) {
+    const Cut c = cut_q(p);
+    const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows;
+    p.tiles = c.tiles;
+    p.splits = c.splits;
+    p.part_stats = (float2*)ws;
+    p.part = (float*)(ws + c.splits * rows * 8);
+    dim3 g;
+    if (int rc = grid(p, c, g)) return rc;
+    by_dim(p.dim, [&](auto d) {
+      constexpr int DP = d.value, W = max_waves<T, DP>();
+      launch<4 * Tile<T, DP>::BYTES>(pct_attend_kernel<T, DP, W>, g, c.waves, s, p);
+    });
+    if (c.splits > 1) pct_attend_join_kernel<T><<<(unsigned)((rows * (p.dim / 4) + 255) / 256), 256, 0, s>>>(p);
+    return policy_launched("attention kernel");
+  }
+  static int backward(AttendParams& p, char* ws, hipStream_t s) {
+    const Cut q = cut_q(p), k = cut_k(p);
+    const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows;
+    p.delta = (float*)ws;
+    p.part = (float*)(ws + (rows * 4 + 255) / 256 * 256);
+    dim3 gq, gk;
+    int rc = grid(p, q, gq);
+    if (!rc) rc = grid(p, k, gk);
+    if (rc) return rc;
+    by_dim(p.dim, [&](auto d) {
+      constexpr int DP = d.value, W = max_waves<T, DP>();
+      p.tiles = q.tiles;
+      p.splits = q.splits;
+      launch<4 * Tile<T, DP>::BYTES>(pct_attend_dq_kernel<T, DP, W>, gq, q.waves, s, p);
+      if (q.splits > 1) {
+        const int64_t n = (int64_t)p.batch * p.q_len * p.heads * p.dim;
+        pct_attend_sum_kernel<T><<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(p.part, n, q.splits, n, (T*)p.dq, (T*)nullptr);
+      }
+      p.tiles = k.tiles;
+      p.splits = k.splits;
+      launch<4 * Tile<T, DP>::BYTES>(pct_attend_dkv_kernel<T, DP, W>, gk, k.waves, s, p);
+      if (k.splits > 1) {
+        const int64_t n = (int64_t)p.batch * p.k_len * p.kv_heads * p.dim;
+        pct_attend_sum_kernel<T><<<dim3((unsigned)((n / 4 + 255) / 256), 2), 256, 0, s>>>(p.part, 2 * n, k.splits, n, (T*)p.dk, (T*)p.dv);
+      }
+    });
+    return policy_launched("attention gradient kernels");
+  }
+};
+
+}  // namespace
+}  // namespace pct
+#endif

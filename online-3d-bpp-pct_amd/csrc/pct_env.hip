@@ -448,6 +448,14 @@ bool is_cand_cap_ok(int c) {
 }
 }  // namespace
 
+namespace pct {  // (for the policy operators' translation units)
+int policy_fail(int code, const char* text) { return fail(code, "%s", text); }
+int policy_launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? PCT_OK : fail(PCT_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+}  // namespace pct
+
 extern "C" {
 
 int pct_abi_version(void) { return PCT_ABI_VERSION; }

@@ -1,0 +1,140 @@
+"""CPU: what the policy operators refuse, and the C ABI of include/pct_policy.h (nothing here launches a kernel)."""
+import ctypes
+import importlib
+import os
+import re
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _pkg():
+    return importlib.import_module("online-3d-bpp-pct_amd")
+
+
+def _ops():
+    return importlib.import_module("online-3d-bpp-pct_amd.policy_ops")
+
+
+def test_header_symbols_are_exported():
+    src = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "pct_policy.h")).read(), flags=re.S)
+    names = sorted(set(re.findall(r"\b(pct_[a-z_]+)\s*\(", src)))
+    assert names == ["pct_attend", "pct_attend_backward", "pct_attend_workspace", "pct_choice_backward", "pct_choice_log_probs",
+                     "pct_choice_pick", "pct_choice_workspace"]
+    L = _ops()._library()
+    assert all(hasattr(L, n) for n in names)
+
+
+def test_pick_refusals():
+    pick = _pkg().pick_actions
+    x = torch.zeros(3, 5)
+    for bad in (torch.zeros(3), torch.zeros(3, 0), torch.zeros(1, 3, 5)):
+        with pytest.raises(ValueError):
+            pick(bad)
+    with pytest.raises(TypeError):
+        pick(x.double())
+    with pytest.raises(TypeError):
+        pick(x, mask=torch.zeros(3, 5, dtype=torch.int64))
+    for mask in (torch.zeros(3, 4), torch.zeros(2, 5), torch.zeros(1, 3, 5)):
+        with pytest.raises(ValueError):
+            pick(x, mask=mask)
+    for noise in (torch.zeros(3, 5).double(), torch.zeros(3, 4), torch.zeros(5)):
+        with pytest.raises(ValueError):
+            pick(x, noise=noise)
+    with pytest.raises(_pkg().PctEnvError, match="no CPU path"):
+        pick(x)
+
+
+def test_log_probs_refusals():
+    f = _pkg().action_log_probs
+    x = torch.zeros(3, 5)
+    with pytest.raises(TypeError):
+        f(x, torch.zeros(3))
+    for ids in (torch.zeros(2, dtype=torch.int64), torch.zeros(3, 65, dtype=torch.int64), torch.zeros(3, 1, 1, dtype=torch.int64)):
+        with pytest.raises(ValueError):
+            f(x, ids)
+    for top in (-1, 65):
+        with pytest.raises(ValueError):
+            f(x, torch.zeros(3, dtype=torch.int64), top=top)
+    with pytest.raises(_pkg().PctEnvError, match="no CPU path"):
+        f(x, torch.zeros(3, dtype=torch.int64))
+
+
+def test_attention_refusals():
+    f = _pkg().cross_attention
+    q, k = torch.zeros(2, 3, 4, 16), torch.zeros(2, 5, 2, 16)
+    for args in ((q[0], k, k), (q, k, k[:, :4]), (q, k[:1], k[:1]), (q[:, :, :3], k, k), (q[..., :8], k, k),
+                 (torch.zeros(2, 3, 4, 12), torch.zeros(2, 5, 2, 12), torch.zeros(2, 5, 2, 12)),
+                 (torch.zeros(2, 3, 4, 136), torch.zeros(2, 5, 2, 136), torch.zeros(2, 5, 2, 136))):
+        with pytest.raises(ValueError):
+            f(*args)
+    with pytest.raises(TypeError):
+        f(q, k.half(), k.half())
+    with pytest.raises(TypeError):
+        f(q.double(), k.double(), k.double())
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError):
+            f(q, k, k, scale=scale)
+    for lengths in (torch.zeros(2), torch.zeros(3, dtype=torch.int32), torch.zeros(2, 1, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            f(q, k, k, key_lengths=lengths)
+    with pytest.raises(ValueError):
+        f(q, k, k, key_mask=torch.zeros(2, 4))
+    with pytest.raises(_pkg().PctEnvError, match="no CPU path"):
+        f(q, k, k)
+
+
+def test_c_entries_refuse_bad_structs():
+    """every refusal returns before anything is enqueued"""
+    ops, lib = _ops(), _pkg()._lib
+    L = ops._library()
+    for fn in (L.pct_choice_pick, L.pct_choice_log_probs, L.pct_choice_backward, L.pct_attend, L.pct_attend_backward):
+        assert fn(None, None) != 0
+    c = ops._Choice()
+    assert L.pct_choice_pick(ctypes.addressof(c), None) != 0 and b"size mismatch" in L.pct_last_error()
+    c.struct_size = ctypes.sizeof(c)
+    c.rows, c.choices = 2, 5
+    assert L.pct_choice_pick(ctypes.addressof(c), None) != 0 and b"null" in L.pct_last_error()
+    c.logits = 4096
+    c.top = 65
+    assert L.pct_choice_log_probs(ctypes.addressof(c), None) != 0
+    c.top, c.dtype = 0, 3
+    assert L.pct_choice_log_probs(ctypes.addressof(c), None) != 0
+    c.dtype, c.choices, c.actions = 0, 1 << 20, 4096
+    assert L.pct_choice_pick(ctypes.addressof(c), None) != 0 and b"workspace" in L.pct_last_error()
+    c.rows = 0
+    assert L.pct_choice_pick(ctypes.addressof(c), None) == lib.PCT_OK
+    a = ops._Attention()
+    a.struct_size = ctypes.sizeof(a)
+    a.batch, a.q_len, a.k_len, a.heads, a.kv_heads, a.dim, a.scale = 1, 2, 3, 3, 2, 16, 1.0
+    assert L.pct_attend(ctypes.addressof(a), None) != 0 and b"multiple" in L.pct_last_error()
+    a.kv_heads, a.dim = 1, 12
+    assert L.pct_attend(ctypes.addressof(a), None) != 0
+    a.dim, a.scale = 16, -1.0
+    assert L.pct_attend(ctypes.addressof(a), None) != 0
+    a.scale, a.key_mask, a.mask_type = 1.0, 4096, 1
+    assert L.pct_attend(ctypes.addressof(a), None) != 0 and b"key_list" in L.pct_last_error()
+    a.key_mask = None
+    assert L.pct_attend(ctypes.addressof(a), None) != 0 and b"null" in L.pct_last_error()
+    a.q = a.k = a.v = a.out = 4104
+    assert L.pct_attend(ctypes.addressof(a), None) != 0 and b"16 bytes" in L.pct_last_error()
+    a.q = a.k = a.v = a.out = 4096
+    assert L.pct_attend_backward(ctypes.addressof(a), None) != 0
+    a.batch = 0
+    assert L.pct_attend(ctypes.addressof(a), None) == lib.PCT_OK
+
+
+def test_workspaces_are_bounded():
+    """a workspace grows with what is split, and nothing is split where the rows fill the chip"""
+    ops = _ops()
+    L = ops._library()
+    assert L.pct_choice_workspace(4096, 131072, 64) == 0 and L.pct_choice_workspace(16, 2048, 20) == 0
+    assert 0 < L.pct_choice_workspace(1, 131072, 64) <= 64 * (32 + 8 * 64)
+    a = ops._Attention()
+    a.struct_size = ctypes.sizeof(a)
+    a.batch, a.q_len, a.k_len, a.heads, a.kv_heads, a.dim, a.scale, a.dtype = 4096, 131, 131, 1, 1, 64, 1.0, 0
+    assert L.pct_attend_workspace(ctypes.addressof(a), 0) == 0
+    a.batch, a.q_len, a.k_len = 1, 1, 16384
+    assert 0 < L.pct_attend_workspace(ctypes.addressof(a), 0) <= 64 * (64 * 4 + 8)
