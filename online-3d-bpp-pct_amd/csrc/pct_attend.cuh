@@ -30,6 +30,17 @@
 
 namespace pct {
 
+// n / d for n < 2^31 by a multiplication: m = 2^32 (2^s - d) / d + 1 with s = ceil(log2 d)
+struct Divisor {
+  uint32_t d, m, s;
+  Divisor() : d(1), m(1), s(0) {}
+  explicit Divisor(uint32_t by) : d(by), s(0) {
+    while (((uint64_t)1 << s) < by) s++;
+    m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - by)) / by + 1);
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
 struct AttendParams {
   const void *q, *k, *v, *d_out, *o;
   int64_t qs[3], ks[3], vs[3], ds[3];  // batch, length, head
@@ -39,6 +50,8 @@ struct AttendParams {
   int batch, q_len, k_len, heads, kv_heads, dim, group, rows;  // rows = q_len * group
   float scale, c;                      // c = scale log2 e
   int tiles, splits;                   // workgroups along the resident rows / along the streamed ones
+  bool tail;                           // the last tiles may find nothing to do
+  Divisor by_tiles, by_splits, by_kv, by_group, by_die;
   void* out;
   float2* stats;                       // [batch, kv_heads, rows]: reference point (log2), sum
   float* delta;                        // [batch, kv_heads, rows]
@@ -70,9 +83,9 @@ template <typename T> struct Type {
 
 // a staged tile: rows of DP elements in 16-byte chunks; a chunk's place within its row is XORed with bits of the row so that 16
 // adjacent rows at one chunk, and 4 adjacent rows at two, meet different banks
-template <typename T, int DP>
+template <typename T, int DP, int R = Type<T>::ROWS>
 struct Tile {
-  static constexpr int CE = Type<T>::CE, CPR = DP / CE, ROWS = Type<T>::ROWS, BYTES = ROWS * DP * (int)sizeof(T);
+  static constexpr int CE = Type<T>::CE, CPR = DP / CE, ROWS = R, BYTES = ROWS * DP * (int)sizeof(T);
   static __device__ __forceinline__ int swz(int row) { return CPR % 16 == 0 ? row & 15 : (CPR % 8 == 0 ? (row >> 1) & 7 : (row >> 2) & 3); }
   static __device__ __forceinline__ int at(int row, int d) { return row * DP + ((d / CE) ^ swz(row)) * CE + d % CE; }
 
@@ -102,15 +115,19 @@ struct Tile {
       return f;
     }
   }
-  // starts the copy of the tile's rows from global memory straight into LDS, 64 chunks to an instruction; the caller waits.
-  // What lies behind `dim` in a row is left as it is (zero from the start).
+  // starts the copy of the rows of two tensors from global memory straight into their tiles, 64 chunks to an instruction; the
+  // caller waits.  What lies behind `dim` in a row is left as it is (zero from the start).
   template <typename Row>
-  static __device__ __forceinline__ void stage(T* t, int dim, int wave, int waves, int lane, Row row_ptr) {
+  static __device__ __forceinline__ void stage2(T* t, T* u, int dim, int wave, int waves, int lane, Row rows) {
+#pragma unroll 4
     for (int i = wave; i < ROWS * CPR / 64; i += waves) {
       const int c = i * 64 + lane, row = c / CPR, d = ((c % CPR) ^ swz(row)) * CE;
-      const T* src = row_ptr(row) + d;
-      if (d < dim)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, LDS_PTR(void, t + i * 64 * CE), 16, 0, 0);
+      const T *a, *b;
+      rows(row, a, b);
+      if (d < dim) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a + d), LDS_PTR(void, t + i * 64 * CE), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + d), LDS_PTR(void, u + i * 64 * CE), 16, 0, 0);
+      }
     }
   }
 };
@@ -150,6 +167,29 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
     *(uint2*)p = make_uint2(pack2<T>(a, b), pack2<T>(c, d));
   }
 }
+// The lane's 16 elements of 32 output elements (register j of an accumulator is element 8 (j / 4) + 4 h + j % 4), f times them:
+// 16-bit elements change places with the other half, so that a lane stores 8 in a row.
+template <typename T>
+__device__ __forceinline__ void store_row(T* dst, const Acc& a, float f, int room, int h) {  // room: elements of the row from dst on
+#pragma unroll
+  for (int j = 0; j < 4; j += sizeof(T) == 4 ? 1 : 2) {
+    if constexpr (sizeof(T) == 4) {
+      const int d = 8 * j + 4 * h;
+      if (d < room) store4<T>(dst + d, a[4 * j] * f, a[4 * j + 1] * f, a[4 * j + 2] * f, a[4 * j + 3] * f);
+    } else {
+      uint32_t x[2], y[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        auto r = __builtin_amdgcn_permlane32_swap(pack2<T>(a[4 * j + 2 * e] * f, a[4 * j + 2 * e + 1] * f),
+                                                  pack2<T>(a[4 * j + 4 + 2 * e] * f, a[4 * j + 5 + 2 * e] * f), false, false);
+        x[e] = r[0];  // of the lower half: elements 0 .. 3 of block j, of the upper: of block j + 1
+        y[e] = r[1];  // elements 4 .. 7
+      }
+      const int d = 8 * (j + h);
+      if (d < room) *(uint4*)(dst + d) = make_uint4(x[0], x[1], y[0], y[1]);
+    }
+  }
+}
 __device__ __forceinline__ float other_half(float v) {
   auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
@@ -167,26 +207,50 @@ __device__ __forceinline__ int acc_row(int j, int h) { return (j & 3) + 8 * (j >
 struct Work { int b, kh, tile, split; };
 // Workgroups go to the 8 dies in turn, and each die has an L2 of its own: the workgroups that stream the same rows are numbered
 // so that they meet on one die.
+// Where part of the tiles may find nothing to do (p.tail), their workgroups come last on each die: numbered side by side with
+// the others they would meet the same compute units every time.  Heads stay side by side, since they share cache lines.
 __device__ __forceinline__ Work decode(const AttendParams& p) {
-  const int total = gridDim.x, die = blockIdx.x & 7, slot = blockIdx.x >> 3, per = total >> 3, rest = total & 7;
-  int w = die * per + (die < rest ? die : rest) + slot;
   Work k;
-  k.tile = w % p.tiles; w /= p.tiles;
-  k.split = w % p.splits; w /= p.splits;
-  k.kh = w % p.kv_heads;
-  k.b = w / p.kv_heads;
+  uint32_t w;
+  if (p.tail) {
+    const uint32_t slot = blockIdx.x >> 3, x = p.by_die.of(slot), bh = (blockIdx.x & 7) * p.by_die.d + (slot - x * p.by_die.d);
+    k.tile = (int)p.by_splits.of(x);
+    k.split = (int)(x - k.tile * p.splits);
+    const bool in = bh < (uint32_t)p.batch * p.kv_heads;
+    k.b = in ? (int)p.by_kv.of(bh) : -1;
+    k.kh = in ? (int)(bh - k.b * p.kv_heads) : 0;
+    return k;
+  }
+  const uint32_t total = gridDim.x, die = blockIdx.x & 7, slot = blockIdx.x >> 3, per = total >> 3, rest = total & 7;
+  w = die * per + (die < rest ? die : rest) + slot;
+  uint32_t x = p.by_tiles.of(w);
+  k.tile = (int)(w - x * p.tiles);
+  w = p.by_splits.of(x);
+  k.split = (int)(x - w * p.splits);
+  k.b = (int)p.by_kv.of(w);
+  k.kh = (int)(w - k.b * p.kv_heads);
   return k;
 }
+// the part of `all` tiles that is split k of n
+__device__ __forceinline__ int split_at(const AttendParams& p, int all, int k) {
+  return p.splits == 1 ? (k ? all : 0) : (int)p.by_splits.of((uint32_t)all * (uint32_t)k);
+}
 
-// element offset of row r = (l, g) of a [batch, length, head, dim] tensor
-__device__ __forceinline__ int64_t row_offset(const int64_t (&s)[3], const AttendParams& p, int b, int kh, int r) {
-  const int l = p.group == 1 ? r : r / p.group, g = r - l * p.group;
-  return b * s[0] + l * s[1] + (int64_t)(kh * p.group + g) * s[2];
+// element offset of row r = (l, g) of a [batch, length, head, dim] tensor behind its head's first row
+__device__ __forceinline__ int64_t row_offset(int64_t ls, int64_t hs, const AttendParams& p, int r) {
+  if (p.group == 1) return r * ls;
+  const int l = (int)p.by_group.of(r), g = r - l * p.group;
+  return l * ls + g * hs;
 }
-__device__ __forceinline__ int64_t out_offset(const AttendParams& p, int b, int kh, int r) {
-  const int l = p.group == 1 ? r : r / p.group, g = r - l * p.group;
-  return (((int64_t)b * p.q_len + l) * p.heads + kh * p.group + g) * p.dim;
+template <typename T>
+__device__ __forceinline__ T* head_of(T* t, const int64_t (&s)[3], const AttendParams& p, const Work& w) {
+  return t + (w.b * s[0] + (int64_t)w.kh * p.group * s[2]);
 }
+// the same in a result, which is contiguous
+__device__ __forceinline__ int64_t out_head(const AttendParams& p, const Work& w) {
+  return ((int64_t)w.b * p.q_len * p.heads + w.kh * p.group) * p.dim;
+}
+__device__ __forceinline__ int64_t out_row(const AttendParams& p, int r) { return row_offset((int64_t)p.heads * p.dim, p.dim, p, r); }
 
 template <int N>
 __device__ __forceinline__ void zero_lds(void* p, int tid, int threads) {
@@ -221,9 +285,9 @@ struct Power {
 };
 
 // ------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int DP, int MAXW>
+template <typename T, int DP, int MAXW, int R>
 __global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
-  using L = Tile<T, DP>;
+  using L = Tile<T, DP, R>;
   constexpr int KT = L::ROWS, SUB = KT / 32, KS = DP / 16, DB = DP / 32;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* const buf = (T*)lds;  // [2][k, v] tiles
@@ -231,35 +295,52 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
   const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6, c32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Work w = decode(p);
-  const int n = allowed_keys(p, w.b), all = (n + KT - 1) / KT;
-  const int t0 = (int)((int64_t)all * w.split / p.splits), t1 = (int)((int64_t)all * (w.split + 1) / p.splits);
   const int row = (w.tile * waves + wave) * 32 + c32;
   const bool active = (w.tile * waves + wave) * 32 < p.rows;
   const int32_t* list = p.list ? p.list + (int64_t)w.b * (p.k_len + 1) + 1 : nullptr;
   const T* kb = (const T*)p.k + w.b * p.ks[0] + w.kh * p.ks[2];
   const T* vb = (const T*)p.v + w.b * p.vs[0] + w.kh * p.vs[2];
 
-  auto key_at = [&](int i) { i = i < n ? i : n - 1; return list ? list[i] : i; };
-  auto stage = [&](int t) {
-    T* k = buf + (t & 1) * 2 * KT * DP;
-    L::stage(k, p.dim, wave, waves, lane, [&](int r) { return kb + keys[t & 1][r] * p.ks[1]; });
-    L::stage(k + KT * DP, p.dim, wave, waves, lane, [&](int r) { return vb + keys[t & 1][r] * p.vs[1]; });
-  };
-  if (p.dim != DP) zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
-  if (t0 < t1) {
-    for (int i = tid; i < KT; i += blockDim.x) {
-      keys[t0 & 1][i] = key_at(t0 * KT + i);
-      keys[(t0 + 1) & 1][i] = key_at((t0 + 1) * KT + i);
-    }
-  }
+  const T* qr = head_of((const T*)p.q, p.qs, p, w) + row_offset(p.qs[1], p.qs[2], p, row);
   Frag<T> qf[KS];
 #pragma unroll
   for (int s = 0; s < KS; s++) {
     const int d = 16 * s + 8 * h;
-    qf[s] = row < p.rows && d < p.dim ? load_frag((const T*)p.q + row_offset(p.qs, p, w.b, w.kh, row) + d) : zero_frag<T>();
+    qf[s] = row < p.rows && d < p.dim ? load_frag(qr + d) : zero_frag<T>();
+  }
+  // (unsplit, the first entries of the list are asked for together with the count: behind it, the first one stands in for them)
+  const bool ahead_of_count = list && p.splits == 1;
+  int early[2 * KT / 64], early0 = 0;
+  if (ahead_of_count) {
+    early0 = list[0];
+#pragma unroll
+    for (int x = 0; x < 2 * KT / 64; x++) {
+      const int i = x * (int)blockDim.x + tid;
+      early[x] = list[i < p.k_len ? i : 0];
+    }
+  }
+  const int n = allowed_keys(p, w.b), all = (n + KT - 1) / KT;
+  const int t0 = split_at(p, all, w.split), t1 = split_at(p, all, w.split + 1);
+  auto key_at = [&](int i) { i = i < n ? i : n - 1; return list ? list[i] : i; };
+  auto stage = [&](int t) {
+    T* k = buf + (t & 1) * 2 * KT * DP;
+    L::stage2(k, k + KT * DP, p.dim, wave, waves, lane, [&](int r, const T*& a, const T*& b) {
+      const int64_t key = keys[t & 1][r];
+      a = kb + key * p.ks[1];
+      b = vb + key * p.vs[1];
+    });
+  };
+  if (p.dim != DP) zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
+  if (t0 < t1) {
+#pragma unroll
+    for (int x = 0; x < 2 * KT / 64; x++) {
+      const int i = x * (int)blockDim.x + tid;
+      if (i < 2 * KT) keys[(t0 + i / KT) & 1][i % KT] = ahead_of_count ? (i < n ? early[x] : early0) : key_at(t0 * KT + i);
+    }
   }
   __syncthreads();
   if (t0 < t1) stage(t0);
+  if (t0 + 1 < t1) stage(t0 + 1);
   Acc o[DB];
 #pragma unroll
   for (int i = 0; i < DB; i++) o[i] = Acc{};
@@ -270,7 +351,7 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
   for (int t = t0; t < t1; t++) {
     tile_barrier();
     int ahead = 0;
-    if (t + 1 < t1) stage(t + 1);
+    if (t > t0 && t + 1 < t1) stage(t + 1);  // (the first two are on their way already)
     if (t + 2 < t1 && tid < KT) ahead = key_at((t + 2) * KT + tid);
     if (active) {
       const T* kt = buf + (t & 1) * 2 * KT * DP;
@@ -343,14 +424,9 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
   }
   const float inv = n > 0 ? 1.f / sum : 0.f;
   if (h == 0 && p.stats) p.stats[at] = n > 0 ? make_float2(ref, sum) : make_float2(0.f, INFINITY);
-  T* dst = (T*)p.out + out_offset(p, w.b, w.kh, row);
+  T* dst = (T*)p.out + out_head(p, w) + out_row(p, row);
 #pragma unroll
-  for (int i = 0; i < DB; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int d = 32 * i + 8 * j + 4 * h;
-      if (d < p.dim) store4<T>(dst + d, o[i][4 * j] * inv, o[i][4 * j + 1] * inv, o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv);
-    }
+  for (int i = 0; i < DB; i++) store_row<T>(dst + 32 * i, o[i], inv, p.dim - 32 * i, h);
 }
 
 // joins the splits of the forward pass: a thread to 4 elements of a row
@@ -375,7 +451,8 @@ __global__ __launch_bounds__(256) void pct_attend_join_kernel(AttendParams p) {
   const bool none = allowed_keys(p, bh / p.kv_heads) == 0;
   const float inv = none ? 0.f : 1.f / sum;
   if (d == 0 && p.stats) p.stats[at] = none ? make_float2(0.f, INFINITY) : make_float2(ref, sum);
-  store4<T>((T*)p.out + out_offset(p, bh / p.kv_heads, bh % p.kv_heads, r) + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  const Work w = {bh / p.kv_heads, bh % p.kv_heads, 0, 0};
+  store4<T>((T*)p.out + out_head(p, w) + out_row(p, r) + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 // P of the backward pass: float32 keeps the forward's reference point and sum apart (their logarithm's rounding would be a
@@ -394,19 +471,18 @@ __device__ __forceinline__ float p_value(float s, float c, float2 t) {
 
 // ---------------------------------------------------------------------------------------------------------------- dq, D
 // D_r = dO_r . O_r, where O_r has been rounded to the tensors' type: over many keys that error vanishes beside dP, over few it
-// would not, so where all keys fit one tile D is summed from P dP itself.
+// would not, so where all keys fit one tile of 16-bit elements D is summed from P dP itself.
 template <typename T, int DP, int MAXW>
 __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p) {
   using L = Tile<T, DP>;
   constexpr int KT = L::ROWS, SUB = KT / 32, KS = DP / 16, DB = DP / 32;
+  constexpr bool EXACT = sizeof(T) == 2;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* const buf = (T*)lds;
   __shared__ int keys[2][KT];
   const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6, c32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Work w = decode(p);
-  const int n = allowed_keys(p, w.b), all = (n + KT - 1) / KT;
-  const int t0 = (int)((int64_t)all * w.split / p.splits), t1 = (int)((int64_t)all * (w.split + 1) / p.splits);
   const int row = (w.tile * waves + wave) * 32 + c32;
   const bool active = (w.tile * waves + wave) * 32 < p.rows;
   const int32_t* list = p.list ? p.list + (int64_t)w.b * (p.k_len + 1) + 1 : nullptr;
@@ -414,37 +490,62 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p
   const T* vb = (const T*)p.v + w.b * p.vs[0] + w.kh * p.vs[2];
   const int64_t at = ((int64_t)w.b * p.kv_heads + w.kh) * p.rows + row;
 
-  auto key_at = [&](int i) { i = i < n ? i : n - 1; return list ? list[i] : i; };
-  auto stage = [&](int t) {
-    T* k = buf + (t & 1) * 2 * KT * DP;
-    L::stage(k, p.dim, wave, waves, lane, [&](int r) { return kb + keys[t & 1][r] * p.ks[1]; });
-    L::stage(k + KT * DP, p.dim, wave, waves, lane, [&](int r) { return vb + keys[t & 1][r] * p.vs[1]; });
-  };
-  if (p.dim != DP) zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
-  if (t0 < t1) {
-    for (int i = tid; i < KT; i += blockDim.x) {
-      keys[t0 & 1][i] = key_at(t0 * KT + i);
-      keys[(t0 + 1) & 1][i] = key_at((t0 + 1) * KT + i);
-    }
-  }
+  const T* qr = head_of((const T*)p.q, p.qs, p, w) + row_offset(p.qs[1], p.qs[2], p, row);
+  const T* dr = head_of((const T*)p.d_out, p.ds, p, w) + row_offset(p.ds[1], p.ds[2], p, row);
   Frag<T> qf[KS], df[KS];
-  float D = 0.f;
-  float2 st = make_float2(INFINITY, 0.f);
-  if (row < p.rows && n > 0) st = p_terms<T>(p.stats[at]);
 #pragma unroll
   for (int s = 0; s < KS; s++) {
     const int d = 16 * s + 8 * h;
     const bool in = row < p.rows && d < p.dim;
-    qf[s] = in ? load_frag((const T*)p.q + row_offset(p.qs, p, w.b, w.kh, row) + d) : zero_frag<T>();
-    df[s] = in ? load_frag((const T*)p.d_out + row_offset(p.ds, p, w.b, w.kh, row) + d) : zero_frag<T>();
-    if (in && n > KT) {
-      const Frag<T> of = load_frag((const T*)p.o + out_offset(p, w.b, w.kh, row) + d);
+    qf[s] = in ? load_frag(qr + d) : zero_frag<T>();
+    df[s] = in ? load_frag(dr + d) : zero_frag<T>();
+  }
+  float2 st = row < p.rows ? p.stats[at] : make_float2(INFINITY, INFINITY);
+  // (unsplit, the first entries of the list are asked for together with the count: behind it, the first one stands in for them)
+  const bool ahead_of_count = list && p.splits == 1;
+  int early[2 * KT / 64], early0 = 0;
+  if (ahead_of_count) {
+    early0 = list[0];
 #pragma unroll
-      for (int e = 0; e < 8; e++) D = fmaf((float)df[s][e], (float)of[e], D);
+    for (int x = 0; x < 2 * KT / 64; x++) {
+      const int i = x * (int)blockDim.x + tid;
+      early[x] = list[i < p.k_len ? i : 0];
+    }
+  }
+  const int n = allowed_keys(p, w.b), all = (n + KT - 1) / KT;
+  const int t0 = split_at(p, all, w.split), t1 = split_at(p, all, w.split + 1);
+  auto key_at = [&](int i) { i = i < n ? i : n - 1; return list ? list[i] : i; };
+  auto stage = [&](int t) {
+    T* k = buf + (t & 1) * 2 * KT * DP;
+    L::stage2(k, k + KT * DP, p.dim, wave, waves, lane, [&](int r, const T*& a, const T*& b) {
+      const int64_t key = keys[t & 1][r];
+      a = kb + key * p.ks[1];
+      b = vb + key * p.vs[1];
+    });
+  };
+  if (p.dim != DP) zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
+  if (t0 < t1) {
+#pragma unroll
+    for (int x = 0; x < 2 * KT / 64; x++) {
+      const int i = x * (int)blockDim.x + tid;
+      if (i < 2 * KT) keys[(t0 + i / KT) & 1][i % KT] = ahead_of_count ? (i < n ? early[x] : early0) : key_at(t0 * KT + i);
     }
   }
   __syncthreads();
   if (t0 < t1) stage(t0);
+  if (t0 + 1 < t1) stage(t0 + 1);
+  st = p_terms<T>(st);
+  float D = 0.f;
+  if (row < p.rows && n > 0 && !(EXACT && n <= KT)) {
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const int d = 16 * s + 8 * h;
+      if (d >= p.dim) break;
+      const Frag<T> of = load_frag((const T*)p.o + out_head(p, w) + out_row(p, row) + d);
+#pragma unroll
+      for (int e = 0; e < 8; e++) D = fmaf((float)df[s][e], (float)of[e], D);
+    }
+  }
   Acc dq[DB];
 #pragma unroll
   for (int i = 0; i < DB; i++) dq[i] = Acc{};
@@ -464,12 +565,12 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p
   for (int t = t0; t < t1; t++) {
     tile_barrier();
     int ahead = 0;
-    if (t + 1 < t1) stage(t + 1);
+    if (t > t0 && t + 1 < t1) stage(t + 1);  // (the first two are on their way already)
     if (t + 2 < t1 && tid < KT) ahead = key_at((t + 2) * KT + tid);
     if (active) {
       const T* kt = buf + (t & 1) * 2 * KT * DP;
       const T* vt = kt + KT * DP;
-      if (n <= KT) {
+      if (EXACT && n <= KT) {
 #pragma unroll 1
         for (int i = 0; i < SUB; i++) {
           Acc s, dp;
@@ -512,18 +613,13 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p
   if (row >= p.rows) return;
   if (h == 0 && t0 == 0 && t1 > 0) p.delta[at] = D;  // (one split of them has the first tile; without keys nobody reads it)
   const float f = Type<T>::F16 ? p.scale * __builtin_amdgcn_exp2f(-(float)power.e - p_lift<T>()) : p.scale;
-  float* part = p.splits > 1 ? p.part + (int64_t)w.split * p.batch * p.q_len * p.heads * p.dim + out_offset(p, w.b, w.kh, row) : nullptr;
-  T* dst = (T*)p.dq + out_offset(p, w.b, w.kh, row);
+  float* part = p.splits > 1 ? p.part + (int64_t)w.split * p.batch * p.q_len * p.heads * p.dim + out_head(p, w) + out_row(p, row) : nullptr;
+  T* dst = (T*)p.dq + out_head(p, w) + out_row(p, row);
 #pragma unroll
-  for (int i = 0; i < DB; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int d = 32 * i + 8 * j + 4 * h;
-      if (d >= p.dim) continue;
-      const float a = dq[i][4 * j] * f, b = dq[i][4 * j + 1] * f, c = dq[i][4 * j + 2] * f, e = dq[i][4 * j + 3] * f;
-      if (part) *(float4*)(part + d) = make_float4(a, b, c, e);
-      else store4<T>(dst + d, a, b, c, e);
-    }
+  for (int i = 0; i < DB; i++) {
+    if (part) store_row<float>(part + 32 * i, dq[i], f, p.dim - 32 * i, h);
+    else store_row<T>(dst + 32 * i, dq[i], f, p.dim - 32 * i, h);
+  }
 }
 
 // --------------------------------------------------------------------------------------------------------------- dk, dv
@@ -537,43 +633,66 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams 
   const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6, c32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Work w = decode(p);
-  const int n = allowed_keys(p, w.b);
-  const int first = (w.tile * waves + wave) * 32, i = first + c32;  // place in the list
-  const bool active = first < n, valid = i < n;
-  const bool any = w.tile * waves * 32 < n;  // (of the workgroup)
-  const int all = any ? (p.rows + QT - 1) / QT : 0;
-  const int t0 = (int)((int64_t)all * w.split / p.splits), t1 = (int)((int64_t)all * (w.split + 1) / p.splits);
+  if (w.b < 0) return;
   const int32_t* list = p.list ? p.list + (int64_t)w.b * (p.k_len + 1) + 1 : nullptr;
+  const int first = (w.tile * waves + wave) * 32, i = first + c32;  // place in the list
   const int key = i < p.k_len ? (list ? list[i] : i) : 0;
+  const int n = allowed_keys(p, w.b);
+  const bool active = first < n, valid = i < n;
+  if (w.tile * waves * 32 >= n) return;  // (the whole workgroup; pct_attend_clear_kernel writes the rows of such keys)
+  const int all = (p.rows + QT - 1) / QT;
+  const int t0 = split_at(p, all, w.split), t1 = split_at(p, all, w.split + 1);
+  const T* qb = head_of((const T*)p.q, p.qs, p, w);
+  const T* db = head_of((const T*)p.d_out, p.ds, p, w);
   const float2* stats = p.stats + ((int64_t)w.b * p.kv_heads + w.kh) * p.rows;
   const float* delta = p.delta + ((int64_t)w.b * p.kv_heads + w.kh) * p.rows;
 
   auto stage = [&](int t) {
     T* q = buf + (t & 1) * 2 * QT * DP;
     auto at = [&](int r) { r += t * QT; return r < p.rows ? r : p.rows - 1; };
-    L::stage(q, p.dim, wave, waves, lane, [&](int r) { return (const T*)p.q + row_offset(p.qs, p, w.b, w.kh, at(r)); });
-    L::stage(q + QT * DP, p.dim, wave, waves, lane, [&](int r) { return (const T*)p.d_out + row_offset(p.ds, p, w.b, w.kh, at(r)); });
+    L::stage2(q, q + QT * DP, p.dim, wave, waves, lane, [&](int r, const T*& a, const T*& b) {
+      const int x = at(r), l = p.group == 1 ? x : (int)p.by_group.of(x), g = x - l * p.group;
+      a = qb + l * p.qs[1] + g * p.qs[2];
+      b = db + l * p.ds[1] + g * p.ds[2];
+    });
   };
-  auto put_terms = [&](int t) {
-    for (int r = tid; r < QT; r += blockDim.x) {
-      const int row = t * QT + r;
-      const float2 x = row < p.rows ? p_terms<T>(stats[row]) : make_float2(INFINITY, 0.f);
-      terms[t & 1][0][r] = x.x;
-      terms[t & 1][1][r] = x.y;
-      terms[t & 1][2][r] = row < p.rows ? delta[row] : 0.f;
+  // (a workgroup has at least 64 threads: one to a staged row)
+  struct Terms { float2 p; float d; };
+  auto get_terms = [&](int t) {
+    const int row = t * QT + tid;
+    Terms x = {make_float2(INFINITY, INFINITY), 0.f};
+    if (tid < QT && row < p.rows) { x.p = stats[row]; x.d = delta[row]; }
+    return x;
+  };
+  auto put_terms = [&](int t, const Terms& y) {
+    if (tid < QT) {
+      const float2 x = p_terms<T>(y.p);
+      terms[t & 1][0][tid] = x.x;
+      terms[t & 1][1][tid] = x.y;
+      terms[t & 1][2][tid] = y.d;
     }
   };
-  if (p.dim != DP) zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
-  Frag<T> kf[KS], vf[KS];
-#pragma unroll
-  for (int s = 0; s < KS; s++) {
-    const int d = 16 * s + 8 * h;
-    const bool in = valid && d < p.dim;
-    kf[s] = in ? load_frag((const T*)p.k + w.b * p.ks[0] + key * p.ks[1] + w.kh * p.ks[2] + d) : zero_frag<T>();
-    vf[s] = in ? load_frag((const T*)p.v + w.b * p.vs[0] + key * p.vs[1] + w.kh * p.vs[2] + d) : zero_frag<T>();
+  if (p.dim != DP) {
+    zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
+    __syncthreads();
   }
-  __syncthreads();
-  if (t0 < t1) { stage(t0); put_terms(t0); }
+  Terms next = {};
+  Frag<T> kf[KS], vf[KS];
+  if (t0 < t1) {
+    const Terms x = get_terms(t0);
+    next = get_terms(t0 + 1);
+    stage(t0);
+    if (t0 + 1 < t1) stage(t0 + 1);
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const int d = 16 * s + 8 * h;
+      const bool in = valid && d < p.dim;
+      kf[s] = in ? load_frag((const T*)p.k + w.b * p.ks[0] + key * p.ks[1] + w.kh * p.ks[2] + d) : zero_frag<T>();
+      vf[s] = in ? load_frag((const T*)p.v + w.b * p.vs[0] + key * p.vs[1] + w.kh * p.vs[2] + d) : zero_frag<T>();
+    }
+    put_terms(t0, x);
+    put_terms(t0 + 1, next);
+  }
   Acc dk[DB], dv[DB];
 #pragma unroll
   for (int d = 0; d < DB; d++) { dk[d] = Acc{}; dv[d] = Acc{}; }
@@ -581,8 +700,12 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams 
   power.start();
   for (int t = t0; t < t1; t++) {
     tile_barrier();
-    if (t + 1 < t1) { stage(t + 1); put_terms(t + 1); }
-    if (!active) continue;
+    const bool more = t > t0 && t + 1 < t1;
+    if (more) {
+      next = get_terms(t + 1);
+      stage(t + 1);
+    }
+    if (active) {
     const T* qt = buf + (t & 1) * 2 * QT * DP;
     const T* dt = qt + QT * DP;
 #pragma unroll 1
@@ -624,33 +747,44 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams 
         }
       }
     }
+    }
+    if (more) put_terms(t + 1, next);
   }
-  if (i >= p.k_len) return;
+  if (!valid) return;
   const float fk = Type<T>::F16 ? p.scale * __builtin_amdgcn_exp2f(-(float)power.e - p_lift<T>()) : p.scale;
   const float fv = __builtin_amdgcn_exp2f(-p_lift<T>());
-  const int64_t at = (((int64_t)w.b * p.k_len + key) * p.kv_heads + w.kh) * p.dim;
+  const int64_t at = ((int64_t)w.b * p.k_len * p.kv_heads + w.kh) * p.dim + key * ((int64_t)p.kv_heads * p.dim);
   const int64_t whole = (int64_t)p.batch * p.k_len * p.kv_heads * p.dim;
   float* part = p.splits > 1 ? p.part + (int64_t)w.split * 2 * whole + at : nullptr;
 #pragma unroll
-  for (int x = 0; x < DB; x++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int d = 32 * x + 8 * j + 4 * h;
-      if (d >= p.dim) continue;
-      float k4[4], v4[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        k4[e] = valid ? dk[x][4 * j + e] * fk : 0.f;
-        v4[e] = valid ? dv[x][4 * j + e] * fv : 0.f;
-      }
-      if (part) {
-        *(float4*)(part + d) = make_float4(k4[0], k4[1], k4[2], k4[3]);
-        *(float4*)(part + whole + d) = make_float4(v4[0], v4[1], v4[2], v4[3]);
-      } else {
-        store4<T>((T*)p.dk + at + d, k4[0], k4[1], k4[2], k4[3]);
-        store4<T>((T*)p.dv + at + d, v4[0], v4[1], v4[2], v4[3]);
-      }
+  for (int x = 0; x < DB; x++) {
+    const int room = p.dim - 32 * x;
+    if (part) {
+      store_row<float>(part + 32 * x, dk[x], fk, room, h);
+      store_row<float>(part + whole + 32 * x, dv[x], fv, room, h);
+    } else {
+      store_row<T>((T*)p.dk + at + 32 * x, dk[x], fk, room, h);
+      store_row<T>((T*)p.dv + at + 32 * x, dv[x], fv, room, h);
     }
+  }
+}
+
+// clears dk and dv of the keys that are not allowed, all heads of one at a time: a workgroup to a batch, 16 bytes to a thread
+template <typename T>
+__global__ __launch_bounds__(256) void pct_attend_clear_kernel(AttendParams p, int chunks) {
+  const int b = blockIdx.x, n = allowed_keys(p, b);
+  const int32_t* list = p.list ? p.list + (int64_t)b * (p.k_len + 1) + 1 : nullptr;
+  const int64_t bytes = (int64_t)p.kv_heads * p.dim * (int64_t)sizeof(T), base = b * p.k_len * bytes;
+  const int per = (int)(bytes / 16), rows = p.k_len - n;
+  // (a row's chunks are shared out in powers of two of threads, so that no division is needed)
+  const int x0 = threadIdx.x % chunks;
+  for (int r = threadIdx.x / chunks + blockIdx.y * (256 / chunks); r < rows; r += gridDim.y * (256 / chunks)) {
+    const int64_t at = base + (list ? list[n + r] : n + r) * bytes;
+    for (int x = x0; x < per; x += chunks) {
+      *(uint4*)((char*)p.dk + at + 16 * x) = make_uint4(0, 0, 0, 0);
+      *(uint4*)((char*)p.dv + at + 16 * x) = make_uint4(0, 0, 0, 0);
+    }
+  }
 }
 
 // adds the splits' partial gradients, laid out as the results are: 4 elements to a thread
@@ -668,7 +802,7 @@ __global__ __launch_bounds__(256) void pct_attend_sum_kernel(const float* part, 
 
 // How the work is cut.  Resident rows: 32 to a wavefront, as many wavefronts to a workgroup as there are rows for (they share a
 // staged tile), but fewer while that leaves compute units without a workgroup.  Streamed rows: split over workgroups until
-// about four wavefronts per compute unit are there, in parts of at least two tiles; the partial results are joined after.
+// about eight wavefronts per compute unit are there, in parts of at least two tiles; the partial results are joined after.
 struct Cut { int waves, tiles, splits; };
 inline Cut cut(int64_t resident, int64_t streamed_tiles, int64_t heads, int max_waves) {
   const int64_t t = (resident + 31) / 32;
@@ -678,7 +812,7 @@ inline Cut cut(int64_t resident, int64_t streamed_tiles, int64_t heads, int max_
     w = (w + 1) / 2;
     blocks = (t + w - 1) / w;
   }
-  int64_t s = (1024 + heads * t - 1) / (heads * t);
+  int64_t s = (2048 + heads * t - 1) / (heads * t);
   s = s < streamed_tiles / 2 ? s : streamed_tiles / 2;
   s = s < 1 ? 1 : (s > 64 ? 64 : s);
   return Cut{(int)w, (int)blocks, (int)s};
@@ -702,69 +836,92 @@ template <typename T> struct Attend {
     if (dim <= 96) return f(std::integral_constant<int, 96>());
     return f(std::integral_constant<int, 128>());
   }
-  static Cut cut_q(const AttendParams& p) {
-    const int mw = by_dim(p.dim, [](auto d) { return max_waves<T, d.value>(); });
+  // Of few wavefronts to a head, small workgroups make better use of the chip: they wait for each other less, and where a part
+  // of unknown size of a short masked row is allowed, those behind it end at once.  Measured (4096 x 131 x 131, float32, a third
+  // of the keys allowed / 2048 x 4 heads x 200 x 401, bfloat16), with up to 8, 4, 2 wavefronts: forward 224, 168, 192 / 138, 128,
+  // 145 us; dq 342, 315, 263 / 215, 202, 227; dk and dv 481, 612, 305 / 460, 481, 305.  Of many (4 x 16 heads x 2048 x 4096) 8
+  // are the best by 5 to 10 %.
+  static Cut cut_q(const AttendParams& p, bool dq) {
+    int mw = by_dim(p.dim, [](auto d) { return max_waves<T, d.value>(); });
+    if (p.rows <= 512) mw = dq && sizeof(T) == 4 ? 2 : 4;
     return cut(p.rows, (p.k_len + Type<T>::ROWS - 1) / Type<T>::ROWS, (int64_t)p.batch * p.kv_heads, mw);
   }
   static Cut cut_k(const AttendParams& p) {
-    const int mw = by_dim(p.dim, [](auto d) { return max_waves<T, d.value>(); });
+    int mw = by_dim(p.dim, [](auto d) { return max_waves<T, d.value>(); });
+    if (p.k_len <= 512) mw = p.list || p.lengths ? 2 : 4;
     return cut(p.k_len, (p.rows + Type<T>::ROWS - 1) / Type<T>::ROWS, (int64_t)p.batch * p.kv_heads, mw);
   }
   static int64_t workspace(const AttendParams& p, bool backward) {
     const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows;
-    const Cut q = cut_q(p);
+    const Cut q = cut_q(p, backward);
     if (!backward) return q.splits > 1 ? q.splits * rows * (8 + 4 * (int64_t)p.dim) : 0;
     const Cut k = cut_k(p);
     const int64_t a = q.splits > 1 ? q.splits * rows * p.dim * 4 : 0;
     const int64_t b = k.splits > 1 ? k.splits * 2 * (int64_t)p.batch * p.k_len * p.kv_heads * p.dim * 4 : 0;
     return (rows * 4 + 255) / 256 * 256 + (a > b ? a : b);
   }
-  static int grid(const AttendParams& p, const Cut& c, dim3& g) {
-    const int64_t n = (int64_t)c.tiles * c.splits * p.batch * p.kv_heads;
+  static void set(AttendParams& p, const Cut& c, bool tail) {
+    p.tiles = c.tiles;
+    p.splits = c.splits;
+    p.tail = tail;
+    p.by_tiles = Divisor(c.tiles);
+    p.by_splits = Divisor(c.splits);
+    p.by_kv = Divisor(p.kv_heads);
+    p.by_group = Divisor(p.group);
+    p.by_die = Divisor((unsigned)(((int64_t)p.batch * p.kv_heads + 7) / 8));
+  }
+  static bool tail(const AttendParams& p) { return (p.list || p.lengths) && p.k_len <= 512; }
+  static int grid(const AttendParams& p, const Cut& c, bool by_die, dim3& g) {
+    const int64_t heads = (int64_t)p.batch * p.kv_heads, n = (int64_t)c.tiles * c.splits * (by_die ? (heads + 7) / 8 * 8 : heads);
     if (n * c.waves * 64 >= (int64_t)1 << 32) return policy_fail(PCT_ERR_UNSUPPORTED, "attention: more workgroups than a launch can hold");
     g = dim3((unsigned)n);
     return PCT_OK;
   }
   static int forward(AttendParams& p, char* ws, hipStream_t s) {
-    const Cut c = cut_q(p);
+    const Cut c = cut_q(p, false);
     const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows;
-    p.tiles = c.tiles;
-    p.splits = c.splits;
+    set(p, c, false);
     p.part_stats = (float2*)ws;
     p.part = (float*)(ws + c.splits * rows * 8);
     dim3 g;
-    if (int rc = grid(p, c, g)) return rc;
+    if (int rc = grid(p, c, false, g)) return rc;
     by_dim(p.dim, [&](auto d) {
       constexpr int DP = d.value, W = max_waves<T, DP>();
-      launch<4 * Tile<T, DP>::BYTES>(pct_attend_kernel<T, DP, W>, g, c.waves, s, p);
+      // a lone wavefront or two are bound by what is in flight: smaller tiles let more of them onto a compute unit
+      if (c.waves <= 2) launch<4 * Tile<T, DP, 32>::BYTES>(pct_attend_kernel<T, DP, W, 32>, g, c.waves, s, p);
+      else launch<4 * Tile<T, DP>::BYTES>(pct_attend_kernel<T, DP, W, Type<T>::ROWS>, g, c.waves, s, p);
     });
     if (c.splits > 1) pct_attend_join_kernel<T><<<(unsigned)((rows * (p.dim / 4) + 255) / 256), 256, 0, s>>>(p);
     return policy_launched("attention kernel");
   }
   static int backward(AttendParams& p, char* ws, hipStream_t s) {
-    const Cut q = cut_q(p), k = cut_k(p);
+    const Cut q = cut_q(p, true), k = cut_k(p);
     const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows;
     p.delta = (float*)ws;
     p.part = (float*)(ws + (rows * 4 + 255) / 256 * 256);
     dim3 gq, gk;
-    int rc = grid(p, q, gq);
-    if (!rc) rc = grid(p, k, gk);
+    int rc = grid(p, q, false, gq);
+    if (!rc) rc = grid(p, k, tail(p), gk);
     if (rc) return rc;
     by_dim(p.dim, [&](auto d) {
       constexpr int DP = d.value, W = max_waves<T, DP>();
-      p.tiles = q.tiles;
-      p.splits = q.splits;
+      set(p, q, false);
       launch<4 * Tile<T, DP>::BYTES>(pct_attend_dq_kernel<T, DP, W>, gq, q.waves, s, p);
       if (q.splits > 1) {
         const int64_t n = (int64_t)p.batch * p.q_len * p.heads * p.dim;
         pct_attend_sum_kernel<T><<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(p.part, n, q.splits, n, (T*)p.dq, (T*)nullptr);
       }
-      p.tiles = k.tiles;
-      p.splits = k.splits;
+      set(p, k, tail(p));
       launch<4 * Tile<T, DP>::BYTES>(pct_attend_dkv_kernel<T, DP, W>, gk, k.waves, s, p);
       if (k.splits > 1) {
         const int64_t n = (int64_t)p.batch * p.k_len * p.kv_heads * p.dim;
         pct_attend_sum_kernel<T><<<dim3((unsigned)((n / 4 + 255) / 256), 2), 256, 0, s>>>(p.part, 2 * n, k.splits, n, (T*)p.dk, (T*)p.dv);
+      }
+      if (p.list || p.lengths) {
+        int chunks = 1;  // threads to a row
+        while (chunks < 64 && 2 * chunks * 16 <= p.kv_heads * p.dim * (int)sizeof(T)) chunks *= 2;
+        const int64_t per = p.k_len / (256 / chunks) / 8 + 1;
+        pct_attend_clear_kernel<T><<<dim3(p.batch, (unsigned)(per < 64 ? per : 64)), 256, 0, s>>>(p, chunks);
       }
     });
     return policy_launched("attention gradient kernels");

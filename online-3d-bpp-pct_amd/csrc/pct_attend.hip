@@ -59,10 +59,9 @@ int check_attention(const pct_attention* a, AttendParams& p) {
   if (a->dim < 8 || a->dim > 128 || a->dim % 8) return policy_fail(PCT_ERR_UNSUPPORTED, "attention: dim must be a multiple of 8 up to 128");
   if (!(a->scale > 0.f) || a->scale > 1e30f) return policy_fail(PCT_ERR_INVALID_ARG, "attention: scale must be positive and finite");
   const int64_t rows = (int64_t)a->q_len * (a->heads / a->kv_heads);
-  if (rows >= (int64_t)1 << 30 || a->k_len >= 1 << 30) return policy_fail(PCT_ERR_UNSUPPORTED, "attention: lengths beyond 2^30 rows");
+  if (rows >= (int64_t)1 << 29 || a->k_len >= 1 << 29) return policy_fail(PCT_ERR_UNSUPPORTED, "attention: lengths beyond 2^29 rows");
   if (a->key_mask && (a->mask_type < PCT_MASK_U8 || a->mask_type > PCT_MASK_I32)) return policy_fail(PCT_ERR_INVALID_ARG, "unknown mask type");
   if (a->key_lengths && a->lengths_type != 4 && a->lengths_type != 8) return policy_fail(PCT_ERR_INVALID_ARG, "key lengths must be int32 or int64");
-  if (a->key_mask && a->batch && a->k_len && !a->key_list) return policy_fail(PCT_ERR_INVALID_ARG, "attention: a key mask needs a key_list");
   p = AttendParams{};
   p.q = a->q; p.k = a->k; p.v = a->v; p.d_out = a->d_out; p.o = a->out;
   for (int i = 0; i < 3; i++) { p.qs[i] = a->q_stride[i]; p.ks[i] = a->k_stride[i]; p.vs[i] = a->v_stride[i]; p.ds[i] = a->d_out_stride[i]; }
@@ -79,6 +78,7 @@ int check_attention(const pct_attention* a, AttendParams& p) {
 int check_pointers(const pct_attention* a, bool backward) {
   const int size = a->dtype == PCT_F32 ? 4 : 2;
   const bool q = a->batch && a->q_len, k = a->batch && a->k_len;
+  if (a->key_mask && a->batch && a->k_len && !a->key_list) return policy_fail(PCT_ERR_INVALID_ARG, "attention: a key mask needs a key_list");
   if ((q && (!a->q || !a->out)) || (k && (!a->k || !a->v))) return policy_fail(PCT_ERR_INVALID_ARG, "attention: null tensor");
   if ((q && !aligned16(a->q, a->q_stride, size)) || (k && (!aligned16(a->k, a->k_stride, size) || !aligned16(a->v, a->v_stride, size))))
     return policy_fail(PCT_ERR_INVALID_ARG, "attention: the rows of q, k and v must start on 16 bytes");
