@@ -98,7 +98,7 @@ struct ChoiceParams {
   Mask mask;
   const float* noise;
   int64_t noise_row;
-  int rows, choices, given_count, top, splits, chunk;
+  int rows, choices, given_count, top, splits, chunk, row0;
   const int64_t* given;
   int64_t* actions;
   float *log_probs, *entropy, *top_log_probs;
@@ -155,7 +155,7 @@ __device__ __forceinline__ void finish_row(const ChoiceParams& p, int row, float
 template <typename T, int MASK, int MODE, int VEC, int TEAM>
 __global__ __launch_bounds__(TEAM == 1 ? 256 : 64 * TEAM) void pct_choice_kernel(ChoiceParams p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = TEAM == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  const int row = p.row0 + (TEAM == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x);
   if (row >= p.rows) return;
   const int c0 = TEAM == 1 ? 0 : (int)blockIdx.y * p.chunk;
   const int c1 = TEAM == 1 ? p.choices : min(p.choices - c0, p.chunk) + c0;
@@ -238,13 +238,25 @@ __global__ __launch_bounds__(TEAM == 1 ? 256 : 64 * TEAM) void pct_choice_kernel
       }
     }
     if constexpr (MODE == LOGP_TOP) {
+      // first each lane's own best: the K-th of these 64 bounds the K-th of all, and little is left above it
+      uint64_t mine = 0;
       const float bar = best.least ? key_value(best.least) : -INFINITY;
       if (__ballot(top >= bar && top > -INFINITY)) {
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-          for (int e = 0; e < VEC; e++)
-            best.offer(v[u][e] != -INFINITY ? choice_key(v[u][e], (int)(i0 + u * STEP + e)) : 0, p.top, lane);
+          for (int e = 0; e < VEC; e++) {
+            const uint64_t k = v[u][e] != -INFINITY ? choice_key(v[u][e], (int)(i0 + u * STEP + e)) : 0;
+            mine = k > mine ? k : mine;
+          }
+        best.offer(mine, p.top, lane);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            const uint64_t k = v[u][e] != -INFINITY ? choice_key(v[u][e], (int)(i0 + u * STEP + e)) : 0;
+            if (__ballot(k != mine && k > best.least)) best.offer(k != mine ? k : 0, p.top, lane);
+          }
       }
     }
   }
@@ -289,11 +301,27 @@ __global__ __launch_bounds__(TEAM == 1 ? 256 : 64 * TEAM) void pct_choice_kernel
   finish_row<T, MASK, MODE>(p, row, m, s, t, key, best.list, lane);
 }
 
-// joins the chunks of a row: one wavefront to a row, a lane to a chunk (at most 64)
+// joins the chunks of a row (at most 64, a lane to each); with a top list 8 wavefronts merge the chunks' lists as a tree
 template <typename T, int MASK, int MODE>
-__global__ __launch_bounds__(64) void pct_choice_join_kernel(ChoiceParams p) {
-  const int lane = threadIdx.x, row = blockIdx.x;
+__global__ __launch_bounds__(MODE == LOGP_TOP ? 512 : 64) void pct_choice_join_kernel(ChoiceParams p) {
+  constexpr int TEAM = MODE == LOGP_TOP ? 8 : 1;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = p.row0 + blockIdx.x;
   const char* w = p.ws + (int64_t)row * p.splits * part_bytes(p.top);
+  uint64_t list = 0;
+  if constexpr (MODE == LOGP_TOP) {
+    __shared__ uint64_t sl[TEAM * 64];
+    for (int c = wave; c < p.splits; c += TEAM) {
+      const uint64_t o = lane < p.top ? ((const uint64_t*)(w + c * part_bytes(p.top) + sizeof(Part)))[lane] : 0;
+      list = c < TEAM ? o : merge64(list, o, lane);
+    }
+    for (int half = TEAM / 2; half; half /= 2) {
+      if (wave >= half && wave < 2 * half) sl[wave * 64 + lane] = list;
+      __syncthreads();
+      if (wave < half) list = merge64(list, sl[(wave + half) * 64 + lane], lane);
+    }
+    if (wave) return;
+    if (lane >= p.top) list = 0;
+  }
   Sums a;
   a.start();
   uint64_t key = 0;
@@ -305,14 +333,6 @@ __global__ __launch_bounds__(64) void pct_choice_join_kernel(ChoiceParams p) {
   if (m > -INFINITY) a.raise(m);
   const float s = wave_sum(a.s), t = wave_sum(a.t);
   if (MODE == PICK) key = wave_max_u64(key);
-  uint64_t list = 0;
-  if constexpr (MODE == LOGP_TOP) {
-    for (int c = 0; c < p.splits; c++) {
-      const uint64_t o = lane < p.top ? ((const uint64_t*)(w + c * part_bytes(p.top) + sizeof(Part)))[lane] : 0;
-      list = merge64(list, o, lane);
-    }
-    if (lane >= p.top) list = 0;
-  }
   finish_row<T, MASK, MODE>(p, row, m, s, t, key, list, lane);
 }
 
@@ -320,7 +340,7 @@ struct ChoiceGradParams {
   const void* x;
   int64_t x_row;
   Mask mask;
-  int rows, choices, given_count, top, chunk;
+  int rows, choices, given_count, top, chunk, row0;
   const int64_t *given, *top_actions;
   const float4* stats;
   const float *d_log_probs, *d_entropy, *d_top;
@@ -334,7 +354,7 @@ struct ChoiceGradParams {
 template <typename T, int MASK, int VEC, int TEAM>
 __global__ __launch_bounds__(TEAM == 1 ? 256 : 64 * TEAM) void pct_choice_grad_kernel(ChoiceGradParams p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = TEAM == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  const int row = p.row0 + (TEAM == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x);
   if (row >= p.rows) return;
   const int c0 = TEAM == 1 ? 0 : (int)blockIdx.y * p.chunk;
   const int c1 = TEAM == 1 ? p.choices : min(p.choices - c0, p.chunk) + c0;
@@ -455,15 +475,21 @@ int choice_splits(int rows, int choices) {
 }
 int choice_chunk(int choices, int splits) { return ((choices + splits - 1) / splits + 511) / 512 * 512; }
 
+constexpr int SLICE = 1 << 22;  // rows to a launch, which holds fewer than 2^32 threads; a multiple of a workgroup's rows
+
 template <typename T, int MASK, int MODE>
 void launch_choice(ChoiceParams& p, hipStream_t s) {
-  if (p.choices <= 128) {
-    pct_choice_kernel<T, MASK, MODE, 1, 1><<<(p.rows + 3) / 4, 256, 0, s>>>(p);
-  } else if (p.choices <= 2048) {
-    pct_choice_kernel<T, MASK, MODE, 8, 1><<<(p.rows + 3) / 4, 256, 0, s>>>(p);
-  } else {
-    pct_choice_kernel<T, MASK, MODE, 8, 8><<<dim3(p.rows, p.splits), 512, 0, s>>>(p);
-    if (p.splits > 1) pct_choice_join_kernel<T, MASK, MODE><<<p.rows, 64, 0, s>>>(p);
+  for (p.row0 = 0; p.row0 < p.rows; p.row0 += SLICE) {
+    const int n = p.rows - p.row0 < SLICE ? p.rows - p.row0 : SLICE;
+    if (p.choices <= 128) {
+      pct_choice_kernel<T, MASK, MODE, 1, 1><<<(n + 3) / 4, 256, 0, s>>>(p);
+    } else if (p.choices <= 2048) {
+      pct_choice_kernel<T, MASK, MODE, 8, 1><<<(n + 3) / 4, 256, 0, s>>>(p);
+    } else {
+      pct_choice_kernel<T, MASK, MODE, 8, 8><<<dim3(n, p.splits), 512, 0, s>>>(p);
+      if (p.splits > 1) pct_choice_join_kernel<T, MASK, MODE><<<n, MODE == LOGP_TOP ? 512 : 64, 0, s>>>(p);
+    }
+    if (p.rows - p.row0 <= SLICE) return;  // (row0 + SLICE may pass 2^31)
   }
 }
 template <typename T, int MASK>
@@ -480,14 +506,14 @@ void launch_choice(ChoiceParams& p, int mode, hipStream_t s) {
 }
 template <typename T, int MASK>
 void launch_grad(ChoiceGradParams& p, hipStream_t s) {
-  if (p.choices <= 128) {
-    pct_choice_grad_kernel<T, MASK, 1, 1><<<(p.rows + 3) / 4, 256, 0, s>>>(p);
-  } else if (p.choices <= 2048) {
-    pct_choice_grad_kernel<T, MASK, 8, 1><<<(p.rows + 3) / 4, 256, 0, s>>>(p);
-  } else {
-    const int splits = choice_splits(p.rows, p.choices);
-    p.chunk = choice_chunk(p.choices, splits);
-    pct_choice_grad_kernel<T, MASK, 8, 8><<<dim3(p.rows, splits), 512, 0, s>>>(p);
+  const int splits = choice_splits(p.rows, p.choices);
+  p.chunk = choice_chunk(p.choices, splits);
+  for (p.row0 = 0; p.row0 < p.rows; p.row0 += SLICE) {
+    const int n = p.rows - p.row0 < SLICE ? p.rows - p.row0 : SLICE;
+    if (p.choices <= 128) pct_choice_grad_kernel<T, MASK, 1, 1><<<(n + 3) / 4, 256, 0, s>>>(p);
+    else if (p.choices <= 2048) pct_choice_grad_kernel<T, MASK, 8, 1><<<(n + 3) / 4, 256, 0, s>>>(p);
+    else pct_choice_grad_kernel<T, MASK, 8, 8><<<dim3(n, splits), 512, 0, s>>>(p);
+    if (p.rows - p.row0 <= SLICE) return;
   }
 }
 template <typename T>

@@ -14,6 +14,7 @@ they can be captured into a graph) and never synchronise.  Tensors on the CPU ar
 """
 import collections
 import ctypes
+import functools
 import math
 
 import torch
@@ -28,6 +29,12 @@ _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _MASK = {torch.bool: 1, torch.uint8: 1, torch.int8: 1, torch.float16: 2, torch.bfloat16: 2, torch.float32: 3, torch.int32: 4}
 _INTS = (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8)
 MAX_GIVEN = MAX_TOP = 64
+
+try:  # the handle alone, without a Stream object around it
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
 
 
 class _Choice(ctypes.Structure):
@@ -47,6 +54,9 @@ class _ChoiceGrad(ctypes.Structure):
                 ("top", ctypes.c_int32), ("pad", ctypes.c_int32), ("top_actions", ctypes.c_void_p), ("stats", ctypes.c_void_p),
                 ("d_log_probs", ctypes.c_void_p), ("d_entropy", ctypes.c_void_p), ("d_top_log_probs", ctypes.c_void_p),
                 ("d_logits", ctypes.c_void_p)]
+
+
+_CHOICE_SIZE, _GRAD_SIZE = ctypes.sizeof(_Choice), ctypes.sizeof(_ChoiceGrad)
 
 
 class _Attention(ctypes.Structure):
@@ -83,21 +93,33 @@ def _library():
 
 def _call(fn, args, device):
     """one C call on the device's current stream, with that device current"""
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            _lib.check(fn(ctypes.addressof(args), torch.cuda.current_stream(device).cuda_stream))
+            rc = fn(ctypes.addressof(args), torch.cuda.current_stream(device).cuda_stream)
     else:
-        _lib.check(fn(ctypes.addressof(args), torch.cuda.current_stream(device).cuda_stream))
+        rc = fn(ctypes.addressof(args), _raw_stream(index))
+    if rc:
+        _lib.check(rc)
+
+
+def _once_differentiable(backward):
+    """torch's once_differentiable, but only where a graph of the backward pass is being made"""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return wrapper
 
 
 def _on_gpu(name, *tensors):
     dev = tensors[0].device
     for t in tensors:
-        if t is not None:
+        if t is not None and (not t.is_cuda or t.device != dev):
             if not t.is_cuda:
                 raise PctEnvError("%s runs on an AMD GPU only (a tensor is on %s); there is no CPU path" % (name, t.device))
-            if t.device != dev:
-                raise ValueError("%s: tensors on %s and on %s" % (name, dev, t.device))
+            raise ValueError("%s: tensors on %s and on %s" % (name, dev, t.device))
     return dev
 
 
@@ -168,7 +190,7 @@ def pick_actions(logits, mask=None, noise=None, actions_out=None, log_probs_out=
         L = _library()
         ws_bytes = L.pct_choice_workspace(n, v, 0)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        c = _Choice(ctypes.sizeof(_Choice), _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask), m_row, m_col, m_type, 0, None,
+        c = _Choice(_CHOICE_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask), m_row, m_col, m_type, 0, None,
                     0, 0, _ptr(noise), noise.stride(0) if noise is not None else 0, actions.data_ptr(), log_probs.data_ptr(),
                     entropy.data_ptr(), None, None, None, _ptr(ws), ws_bytes)
         _call(L.pct_choice_pick, c, dev)
@@ -188,7 +210,7 @@ def _log_probs_forward(x, given, mask, top, want_stats):
         L = _library()
         ws_bytes = L.pct_choice_workspace(n, v, top)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        c = _Choice(ctypes.sizeof(_Choice), _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask[0]), mask[1], mask[2], mask[3],
+        c = _Choice(_CHOICE_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask[0]), mask[1], mask[2], mask[3],
                     g, given.data_ptr(), top, 0, None, 0, None, log_probs.data_ptr(), entropy.data_ptr(), _ptr(top_log_probs),
                     _ptr(top_actions), _ptr(stats), _ptr(ws), ws_bytes)
         _call(L.pct_choice_log_probs, c, dev)
@@ -209,7 +231,7 @@ class _LogProbs(torch.autograd.Function):
         return log_probs, entropy
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, d_log_probs, d_entropy, d_top=None, _=None):
         x, given, mask, top_actions, stats = ctx.saved_tensors
         n, v = x.shape
@@ -217,7 +239,7 @@ class _LogProbs(torch.autograd.Function):
         if n:
             d_log_probs, d_entropy, d_top = (None if t is None else t.contiguous() for t in (d_log_probs, d_entropy, d_top))
             m_row, m_col, m_type = ctx.mask_args
-            c = _ChoiceGrad(ctypes.sizeof(_ChoiceGrad), _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask), m_row, m_col, m_type,
+            c = _ChoiceGrad(_GRAD_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask), m_row, m_col, m_type,
                             given.shape[1], given.data_ptr(), 0 if top_actions is None else top_actions.shape[1], 0, _ptr(top_actions),
                             stats.data_ptr(), _ptr(d_log_probs), _ptr(d_entropy), _ptr(d_top), dx.data_ptr())
             _call(_library().pct_choice_backward, c, x.device)
@@ -260,16 +282,22 @@ def action_log_probs(logits, actions, mask=None, top=0):
 def _attention_rows(x):
     """x [batch, length, heads, dim] as the kernels read it -- unit stride along dim, every row on a 16-byte boundary -- itself
     where it is so, else a copy"""
-    per = 16 // x.element_size()
-    if (x.stride(3) == 1 or x.shape[3] == 1) and x.data_ptr() % 16 == 0 and not any(
-            x.stride(i) % per for i in range(3) if x.shape[i] > 1):
-        return x
+    if x.data_ptr() % 16 == 0:
+        if x.is_contiguous():
+            return x
+        per = 16 // x.element_size()
+        if (x.stride(3) == 1 or x.shape[3] == 1) and not any(x.stride(i) % per for i in range(3) if x.shape[i] > 1):
+            return x
     return x.contiguous() if not x.is_contiguous() else x.clone()
 
 
+_Strides = ctypes.c_int64 * 3
+
+
 def _strides(x):
+    s, n = x.stride(), x.shape
     # (the stride of a dimension of one element is arbitrary)
-    return (ctypes.c_int64 * 3)(*(x.stride(i) if x.shape[i] > 1 else 0 for i in range(3)))
+    return _Strides(s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
 
 
 def _attention_struct(q, k, v, mask, lengths, scale, out, stats, key_list):
@@ -324,7 +352,7 @@ class _CrossAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, d_out):
         q, k, v, mask, lengths, out, stats, key_list = ctx.saved_tensors
         m_row, m_col, m_type, scale = ctx.args
