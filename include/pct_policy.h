@@ -92,7 +92,7 @@ typedef struct pct_attention {
   int32_t batch, q_len, k_len, heads, kv_heads, dim; /* heads a multiple of kv_heads; dim a multiple of 8, 8 .. 128 */
   const void *q, *k, *v;                             /* [batch, length, heads, dim], unit stride along dim; rows start on 16 bytes */
   int64_t q_stride[3], k_stride[3], v_stride[3];     /* batch, length, head */
-  const void* key_mask;                              /* [batch, k_len] or NULL */
+  const void* key_mask;                              /* [batch, k_len] or NULL; the backward only looks whether it is NULL */
   int64_t mask_row, mask_col;
   int32_t mask_type;
   int32_t lengths_type;    /* 4: int32, 8: int64 */

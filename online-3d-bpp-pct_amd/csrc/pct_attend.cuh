@@ -62,6 +62,8 @@ struct AttendParams {
 
 namespace {
 
+constexpr float kLowest = -3.402823466e38f;
+
 template <typename T> using Frag = T __attribute__((ext_vector_type(8)));
 typedef float Acc __attribute__((ext_vector_type(16)));
 
@@ -347,7 +349,8 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
   // exponents are taken against `ref`, which follows the maximum only when it is left behind by more than 2^6 (P then stays
   // small enough for every type, and the sums are rarely scaled); float16 lifts P by 2^8 out of its denormals
   constexpr float LIFT = Type<T>::F16 ? 8.f : 0.f;
-  float ref = -INFINITY, sum = 0.f;
+  // (it starts at the lowest number, not at -infinity: a tile of scores that are all -infinity then weighs 0, not NaN)
+  float ref = kLowest, sum = 0.f;
   for (int t = t0; t < t1; t++) {
     tile_barrier();
     int ahead = 0;
@@ -437,17 +440,16 @@ __global__ __launch_bounds__(256) void pct_attend_join_kernel(AttendParams p) {
   if (i >= rows * per) return;
   const int64_t at = i / per;
   const int d = (int)(i % per) * 4, r = (int)(at % p.rows), bh = (int)(at / p.rows);
-  float ref = -INFINITY, sum = 0.f;
+  float ref = kLowest, sum = 0.f;
   for (int s = 0; s < p.splits; s++) ref = fmaxf(ref, p.part_stats[s * rows + at].x);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (ref > -INFINITY)
-    for (int s = 0; s < p.splits; s++) {
-      const float2 st = p.part_stats[s * rows + at];
-      const float f = __builtin_amdgcn_exp2f(st.x - ref);
-      const float4 x = *(const float4*)(p.part + (s * rows + at) * p.dim + d);
-      sum += f * st.y;
-      o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
-    }
+  for (int s = 0; s < p.splits; s++) {
+    const float2 st = p.part_stats[s * rows + at];
+    const float f = __builtin_amdgcn_exp2f(st.x - ref);
+    const float4 x = *(const float4*)(p.part + (s * rows + at) * p.dim + d);
+    sum += f * st.y;
+    o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
+  }
   const bool none = allowed_keys(p, bh / p.kv_heads) == 0;
   const float inv = none ? 0.f : 1.f / sum;
   if (d == 0 && p.stats) p.stats[at] = none ? make_float2(0.f, INFINITY) : make_float2(ref, sum);
@@ -458,6 +460,9 @@ __global__ __launch_bounds__(256) void pct_attend_join_kernel(AttendParams p) {
 // P of the backward pass: float32 keeps the forward's reference point and sum apart (their logarithm's rounding would be a
 // common factor of the row), the others fold them, and float16 lifts P by 2^14 (P <= 1)
 template <typename T> constexpr float p_lift() { return Type<T>::F16 ? 14.f : 0.f; }
+// (a lone key has P = 1: asked for with c = 0 and these terms it is that to the last bit, so that dP - D is 0 as it should be)
+template <typename T>
+__device__ __forceinline__ float2 p_alone() { return make_float2(-p_lift<T>(), 1.f); }
 template <typename T>
 __device__ __forceinline__ float2 p_terms(float2 st) {
   if constexpr (sizeof(T) == 4) return make_float2(st.x, 1.f / st.y);
@@ -471,7 +476,8 @@ __device__ __forceinline__ float p_value(float s, float c, float2 t) {
 
 // ---------------------------------------------------------------------------------------------------------------- dq, D
 // D_r = dO_r . O_r, where O_r has been rounded to the tensors' type: over many keys that error vanishes beside dP, over few it
-// would not, so where all keys fit one tile of 16-bit elements D is summed from P dP itself.
+// would not, so where all keys fit one tile of 16-bit elements D is summed from P dP itself.  So is that of a lone key, in every
+// type: its dS is then exactly 0.
 template <typename T, int DP, int MAXW>
 __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p) {
   using L = Tile<T, DP>;
@@ -534,9 +540,11 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p
   __syncthreads();
   if (t0 < t1) stage(t0);
   if (t0 + 1 < t1) stage(t0 + 1);
-  st = p_terms<T>(st);
+  st = n == 1 ? p_alone<T>() : p_terms<T>(st);
+  const float c = n == 1 ? 0.f : p.c;
+  const bool few = n == 1 || (EXACT && n <= KT);
   float D = 0.f;
-  if (row < p.rows && n > 0 && !(EXACT && n <= KT)) {
+  if (row < p.rows && n > 0 && !few) {
 #pragma unroll
     for (int s = 0; s < KS; s++) {
       const int d = 16 * s + 8 * h;
@@ -560,7 +568,7 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p
       dp = mfma(L::row8(vt, first % KT + c32, 16 * x + 8 * h), df[x], dp);
     }
 #pragma unroll
-    for (int j = 0; j < 16; j++) s[j] = first + acc_row(j, h) < n ? p_value<T>(s[j], p.c, st) : 0.f;
+    for (int j = 0; j < 16; j++) s[j] = first + acc_row(j, h) < n ? p_value<T>(s[j], c, st) : 0.f;
   };
   for (int t = t0; t < t1; t++) {
     tile_barrier();
@@ -570,7 +578,7 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p
     if (active) {
       const T* kt = buf + (t & 1) * 2 * KT * DP;
       const T* vt = kt + KT * DP;
-      if (EXACT && n <= KT) {
+      if (few) {
 #pragma unroll 1
         for (int i = 0; i < SUB; i++) {
           Acc s, dp;
@@ -666,7 +674,7 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams 
   };
   auto put_terms = [&](int t, const Terms& y) {
     if (tid < QT) {
-      const float2 x = p_terms<T>(y.p);
+      const float2 x = n == 1 && t * QT + tid < p.rows ? p_alone<T>() : p_terms<T>(y.p);
       terms[t & 1][0][tid] = x.x;
       terms[t & 1][1][tid] = x.y;
       terms[t & 1][2][tid] = y.d;
@@ -676,6 +684,7 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams 
     zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
     __syncthreads();
   }
+  const float c = n == 1 ? 0.f : p.c;
   Terms next = {};
   Frag<T> kf[KS], vf[KS];
   if (t0 < t1) {
@@ -727,7 +736,7 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams 
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int j = 4 * g + e;
-          p16[j] = p_value<T>(s[j], p.c, make_float2((&a.x)[e], (&b.x)[e]));
+          p16[j] = p_value<T>(s[j], c, make_float2((&a.x)[e], (&b.x)[e]));
           e16[j] = p16[j] * (dp[j] - (&D.x)[e]);
           if (Type<T>::F16) big = fmaxf(big, fabsf(e16[j]));
         }
@@ -771,8 +780,8 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams 
 
 // clears dk and dv of the keys that are not allowed, all heads of one at a time: a workgroup to a batch, 16 bytes to a thread
 template <typename T>
-__global__ __launch_bounds__(256) void pct_attend_clear_kernel(AttendParams p, int chunks) {
-  const int b = blockIdx.x, n = allowed_keys(p, b);
+__global__ __launch_bounds__(256) void pct_attend_clear_kernel(AttendParams p, int chunks, int b0) {
+  const int b = b0 + blockIdx.x, n = allowed_keys(p, b);
   const int32_t* list = p.list ? p.list + (int64_t)b * (p.k_len + 1) + 1 : nullptr;
   const int64_t bytes = (int64_t)p.kv_heads * p.dim * (int64_t)sizeof(T), base = b * p.k_len * bytes;
   const int per = (int)(bytes / 16), rows = p.k_len - n;
@@ -921,7 +930,9 @@ template <typename T> struct Attend {
         int chunks = 1;  // threads to a row
         while (chunks < 64 && 2 * chunks * 16 <= p.kv_heads * p.dim * (int)sizeof(T)) chunks *= 2;
         const int64_t per = p.k_len / (256 / chunks) / 8 + 1;
-        pct_attend_clear_kernel<T><<<dim3(p.batch, (unsigned)(per < 64 ? per : 64)), 256, 0, s>>>(p, chunks);
+        constexpr int SLICE = 1 << 17;  // batches to a launch, which holds fewer than 2^32 threads
+        for (int64_t b = 0; b < p.batch; b += SLICE)
+          pct_attend_clear_kernel<T><<<dim3((unsigned)(p.batch - b < SLICE ? p.batch - b : SLICE), (unsigned)(per < 64 ? per : 64)), 256, 0, s>>>(p, chunks, (int)b);
       }
     });
     return policy_launched("attention gradient kernels");

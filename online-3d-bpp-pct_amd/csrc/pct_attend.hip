@@ -11,11 +11,13 @@ PCT_ATTEND_TYPE(bf16)
 PCT_ATTEND_TYPE(f16)
 
 namespace {
+constexpr int SLICE = 1 << 22;  // batches to a launch, which holds fewer than 2^32 threads
+
 // A batch's keys in the order: allowed ones, then the others, both rising; the count of the allowed ones in front.  One workgroup
 // to a batch reads its mask twice (the second time from L2): to count, and to place.
-__global__ __launch_bounds__(256) void pct_attend_list_kernel(Mask mask, AttendParams p, int32_t* lists) {
+__global__ __launch_bounds__(256) void pct_attend_list_kernel(Mask mask, AttendParams p, int32_t* lists, int b0) {
   __shared__ int part[4];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = b0 + blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int32_t* out = lists + (int64_t)b * (p.k_len + 1);
   p.list = nullptr;
   const int limit = allowed_keys(p, b);  // by the lengths
@@ -123,7 +125,11 @@ int pct_attend(const pct_attention* a, void* stream) {
   const int64_t need = pct::workspace(a, p, false);
   if (need && (!a->workspace || a->workspace_bytes < need)) return pct::policy_fail(PCT_ERR_INVALID_ARG, "the workspace is smaller than pct_attend_workspace() says");
   if (a->key_mask)
-    pct::pct_attend_list_kernel<<<p.batch, 256, 0, s>>>(pct::Mask{a->key_mask, a->mask_row, a->mask_col, a->mask_type}, p, a->key_list);
+    for (int b = 0; b < p.batch; b += pct::SLICE) {
+      pct::pct_attend_list_kernel<<<p.batch - b < pct::SLICE ? p.batch - b : pct::SLICE, 256, 0, s>>>(
+          pct::Mask{a->key_mask, a->mask_row, a->mask_col, a->mask_type}, p, a->key_list, b);
+      if (p.batch - b <= pct::SLICE) break;  // (b + SLICE may pass 2^31)
+    }
   char* ws = (char*)a->workspace;
   return a->dtype == PCT_F32 ? pct::attend_forward_f32(p, ws, s) : (a->dtype == PCT_BF16 ? pct::attend_forward_bf16(p, ws, s) : pct::attend_forward_f16(p, ws, s));
 }

@@ -469,11 +469,15 @@ namespace {
 // at least 4096 (a workgroup's fixed costs are those of about 2000 elements) and, for the join's one lane to a chunk, at most 64.
 int choice_splits(int rows, int choices) {
   if (choices <= 2048) return 1;
-  int s = (1024 + rows - 1) / rows;
-  s = s < (choices + 4095) / 4096 ? s : (choices + 4095) / 4096;
-  return s < 1 ? 1 : (s > 64 ? 64 : s);
+  int64_t s = (1024 + (int64_t)rows - 1) / rows;
+  const int64_t most = ((int64_t)choices + 4095) / 4096;
+  s = s < most ? s : most;
+  return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
 }
-int choice_chunk(int choices, int splits) { return ((choices + splits - 1) / splits + 511) / 512 * 512; }
+int choice_chunk(int choices, int splits) {  // a multiple of 512 unless it is the whole row
+  const int64_t c = (((int64_t)choices + splits - 1) / splits + 511) / 512 * 512;
+  return c < choices ? (int)c : choices;
+}
 
 constexpr int SLICE = 1 << 22;  // rows to a launch, which holds fewer than 2^32 threads; a multiple of a workgroup's rows
 

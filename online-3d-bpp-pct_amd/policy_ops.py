@@ -72,6 +72,8 @@ class _Attention(ctypes.Structure):
                 ("d_k", ctypes.c_void_p), ("d_v", ctypes.c_void_p)]
 
 
+_ATTENTION_SIZE = ctypes.sizeof(_Attention)
+
 _L = None
 
 
@@ -301,21 +303,11 @@ def _strides(x):
 
 
 def _attention_struct(q, k, v, mask, lengths, scale, out, stats, key_list):
+    """mask: (tensor, row stride, column stride, type); the backward reads key_list alone, and says so with any address and type"""
     b, lq, h, d = q.shape
-    a = _Attention()
-    a.struct_size = ctypes.sizeof(_Attention)
-    a.dtype = _DTYPE[q.dtype]
-    a.batch, a.q_len, a.k_len, a.heads, a.kv_heads, a.dim = b, lq, k.shape[1], h, k.shape[2], d
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_stride, a.k_stride, a.v_stride = _strides(q), _strides(k), _strides(v)
-    if mask[0] is not None:
-        a.key_mask, a.mask_row, a.mask_col, a.mask_type = mask[0].data_ptr(), mask[1], mask[2], mask[3]
-        a.key_list = key_list.data_ptr()
-    if lengths is not None:
-        a.key_lengths, a.lengths_type = lengths.data_ptr(), lengths.element_size()
-    a.scale = scale
-    a.out, a.stats = out.data_ptr(), _ptr(stats)
-    return a
+    return _Attention(_ATTENTION_SIZE, _DTYPE[q.dtype], b, lq, k.shape[1], h, k.shape[2], d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                      _strides(q), _strides(k), _strides(v), _ptr(mask[0]), mask[1], mask[2], mask[3],
+                      0 if lengths is None else lengths.element_size(), _ptr(lengths), scale, 0, out.data_ptr(), _ptr(stats), _ptr(key_list))
 
 
 def _workspace(L, a, backward, dev):
@@ -347,15 +339,14 @@ class _CrossAttention(torch.autograd.Function):
         q, k, v = _attention_rows(q), _attention_rows(k), _attention_rows(v)
         out, stats, key_list = _attend_forward(q, k, v, (mask, m_row, m_col, m_type), lengths, scale, True)
         # (the backward reads the list the forward made of the mask, never the mask itself)
-        ctx.save_for_backward(q, k, v, mask, lengths, out, stats, key_list)
-        ctx.args = (m_row, m_col, m_type, scale)
+        ctx.save_for_backward(q, k, v, lengths, out, stats, key_list)
+        ctx.scale = scale
         return out
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, d_out):
-        q, k, v, mask, lengths, out, stats, key_list = ctx.saved_tensors
-        m_row, m_col, m_type, scale = ctx.args
+        q, k, v, lengths, out, stats, key_list = ctx.saved_tensors
         d_out = _attention_rows(d_out)
         dev = q.device
         d_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
@@ -363,7 +354,7 @@ class _CrossAttention(torch.autograd.Function):
         d_v = torch.empty(v.shape, dtype=v.dtype, device=dev)
         if q.shape[0]:
             L = _library()
-            a = _attention_struct(q, k, v, (mask, m_row, m_col, m_type), lengths, scale, out, stats, key_list)
+            a = _attention_struct(q, k, v, (key_list, 0, 0, 4), lengths, ctx.scale, out, stats, key_list)
             a.d_out, a.d_out_stride = d_out.data_ptr(), _strides(d_out)
             a.d_q, a.d_k, a.d_v = d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr()
             ws = _workspace(L, a, 1, dev)  # noqa: F841

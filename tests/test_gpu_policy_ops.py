@@ -379,6 +379,73 @@ def test_attention_empty_sizes():
             assert g.shape == t.shape and not g.any()
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+def test_attention_to_a_lone_key(dtype):
+    """one allowed key: P = 1, so the output is its value, dS is 0 and dv the sum of the output's gradients"""
+    pk = _pkg()
+    for lk, keys in ((1, None), (70, torch.tensor([1, 0, 1, 1]))):
+        q, k, v, do = _qkv((4, 45, lk, 6, 2, 48), dtype, 11)
+        for t in (q, k, v):
+            t.requires_grad_(True)
+        out = pk.cross_attention(q, k, v, key_lengths=None if keys is None else keys.cuda(), scale=3.0)
+        dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+        has = torch.ones(4, dtype=torch.bool) if keys is None else keys > 0
+        want = v.detach()[:, :1].repeat_interleave(3, 2).expand(4, 45, 6, 48) * has.to(v.dtype).cuda()[:, None, None, None]
+        # 1 / sum and the product with it round to 2^-24 each, the result to its type
+        u = torch.finfo(DT[dtype]).eps / 2 + 2.0 ** -22
+        _close(out.detach(), want.double().cpu(), u * want.double().cpu().abs(), "out")
+        assert not dq.any() and not dk.any() and not dv[:, 1:].any()
+        s = do.double().cpu().view(4, 45, 2, 3, 48).sum((1, 3)) * has[:, None, None]
+        size = do.double().cpu().abs().view(4, 45, 2, 3, 48).sum((1, 3))
+        tiny = 2.0 ** -25 if dtype == "f16" else 0.0
+        _close(dv[:, 0], s, torch.finfo(DT[dtype]).eps / 2 * s.abs() + 135 * 2.0 ** -24 * size + tiny, "dv")
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_scores_of_minus_infinity_weigh_nothing(dtype):
+    """allowed keys whose score is -inf come first, fill whole tiles and whole splits; the others share the weight"""
+    pk = _pkg()
+    for lq, lk, first in ((3, 300, 130), (40, 90, 33), (1, 5000, 4000)):
+        q, k, v, _ = _qkv((2, lq, lk, 2, 2, 32), dtype, 12)
+        q = q.abs() + 0.5
+        k[:, :first] = -math.inf
+        out = pk.cross_attention(q, k, v)
+        want = pk.cross_attention(q, k[:, first:], v[:, first:])
+        _, bound = ref.attention(q, k[:, first:], v[:, first:], None, 1 / math.sqrt(32))
+        _close(out, want.double().cpu(), 2 * bound[0], (lq, lk))
+
+
+def test_long_heads_captured():
+    """heads of 128, whose tiles need more shared memory than a launch gets unasked, in a graph with the backward pass"""
+    pk = _pkg()
+    q, k, v, do = _qkv((2, 70, 300, 4, 2, 128), "f32", 13)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    run = lambda: (lambda o: (o.detach(),) + torch.autograd.grad(o, leaves, do))(pk.cross_attention(q, k, v))
+    eager = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for _ in range(3):
+        for t in held:
+            t.detach().fill_(-7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager))
+        eager = run()
+
+
+def test_the_mask_may_change_after_the_forward_pass():
+    """an observation's mask column is overwritten by the next step: the backward reads what the forward made of it"""
+    pk = _pkg()
+    q, k, v, do = _qkv((3, 20, 60, 1, 1, 16), "f32", 14)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    mask = (torch.rand(3, 60, generator=_gen(5)) < 0.5).float().cuda()
+    want = torch.autograd.grad(pk.cross_attention(q, k, v, key_mask=mask), leaves, do)
+    out = pk.cross_attention(q, k, v, key_mask=mask)
+    mask.fill_(1.0)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, do), want))
+
+
 def test_attention_gradient_against_differences():
     pk = _pkg()
     q, k, v, do = _qkv((1, 3, 9, 2, 1, 8), "f32", 6)

@@ -138,3 +138,11 @@ def test_workspaces_are_bounded():
     assert L.pct_attend_workspace(ctypes.addressof(a), 0) == 0
     a.batch, a.q_len, a.k_len = 1, 1, 16384
     assert 0 < L.pct_attend_workspace(ctypes.addressof(a), 0) <= 64 * (64 * 4 + 8)
+
+
+def test_workspace_of_the_longest_rows():
+    """sizes near 2^31 are cut like any others (64 chunks at most, 32 bytes each without a top list)"""
+    L = _ops()._library()
+    for choices in (2 ** 31 - 1, 2 ** 31 - 100, 2 ** 31 - 4096, 2 ** 30):
+        assert L.pct_choice_workspace(1, choices, 0) == 64 * 32
+        assert L.pct_choice_workspace(2 ** 31 - 1, choices, 0) == 0
