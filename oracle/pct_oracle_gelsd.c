@@ -17,7 +17,8 @@
  * BLAS layer is OpenBLAS' hand-written kernels, whose summation orders and fused multiply-adds differ per CPU family
  * (the reference's stability verdicts on tie cases differ between machines for that reason: profiles/r04_lstsq_ondomain.txt).
  * Restated here is the kernel set OpenBLAS dispatches to on AVX-512 hosts ("SkylakeX" -- the build container; it reuses
- * the Haswell dgemv_t / daxpy / dger kernels), read from the disassembly of the bundled library:
+ * the Haswell dgemv_t / daxpy / dger kernels).  Which order each routine sums in and what it fuses shows in its outputs, pair of
+ * terms by pair of terms: tests/golden/check_blas_order.py probes the library and this file so, for both kernel sets:
  *   dnrm2   x87: squares and sums in 80-bit extended precision, four accumulators over blocks of eight
  *           (A: i = 0 mod 4 ... D: i = 3 mod 4), the n mod 8 tail into A, ((C + A) + B) + D, fsqrt, ONE rounding to double
  *   dgemv T rows in groups of four: columns in groups of four by the AVX2 kernel (per column four lanes of FMA chains,
