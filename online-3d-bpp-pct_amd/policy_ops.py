@@ -10,7 +10,10 @@ include/pct_policy.h:
                       and shared key/value heads, differentiable with respect to q, k and v.
 
 All of them run on the current stream of the tensors' device, allocate outputs and workspaces from torch's allocator (so
-they can be captured into a graph) and never synchronise.  Tensors on the CPU are refused: there is no CPU path.
+they can be captured into a graph) and never synchronise.  A tensor that another stream is still writing, or is handed to
+another stream for reuse, is the caller's to order (wait_stream, record_stream), as with torch's own operators.  To capture a
+backward pass, let no eager graph of the same leaves live: their accumulation nodes remember the stream they were made on.
+Tensors on the CPU are refused: there is no CPU path.
 """
 import collections
 import ctypes
@@ -257,7 +260,8 @@ def action_log_probs(logits, actions, mask=None, top=0):
     An id of -1 stands for "none": log-probability 0, no gradient.  A choice that is not allowed has -inf and takes no
     gradient; an id outside of [-1, V) has NaN.  A row that allows nothing has log-probabilities and entropy 0 and a zero
     gradient.  Alternatives come in falling order, the lower index first among equal logits; where fewer than K choices are
-    allowed the rest is -inf with action -1."""
+    allowed the rest is -inf with action -1.  The backward pass reads the logits and the mask again: neither may have been
+    written over by then."""
     _check_logits("action_log_probs", logits)
     n = logits.shape[0]
     if actions.dtype not in _INTS:
@@ -370,6 +374,8 @@ def cross_attention(q, k, v, key_mask=None, key_lengths=None, scale=None):
     Key j of batch b is allowed where `key_mask` [B, Lk] (any strides: the observation's mask column will do) is not zero and
     j < `key_lengths`[b] (int32 or int64 [B]; values outside of [0, Lk] count as the nearer end).  What stands in keys and
     values that are not allowed does not matter, NaN included.  A batch that allows no key gives zeros and takes no gradient.
+    Lk, and Lq * H / Hk, are below 2^29, and a call is refused whose launch would hold more than 2^32 threads (some 2^26
+    heads times groups of 32 rows).  The mask may be written over once the call has returned to its stream's order.
     `scale` is positive, 1 / sqrt(D) if not given.  q, k, v and the output's gradient are read where they are if their rows
     are contiguous and start on 16 bytes, else from a copy."""
     name = "cross_attention"

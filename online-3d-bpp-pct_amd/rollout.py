@@ -8,9 +8,12 @@ into `obs[t + 1]`, its reward into `rewards[t]` and 1 - done into `masks[t + 1]`
 pct_bind_rollout_slot + pct_step_index): one launch per step, no copy kernels, nothing leaves the GPU.  What
 the policy produces (action index, log-probability) is the caller's to keep; `RolloutSlots.step_env` records
 them beside the slot.  The tensor names and shapes are the trainer's contract (storage.py:5-11); the update rules
-`after_update` / `compute_returns` are storage.py:41-50, restated.
+`after_update` / `compute_returns` are storage.py:41-50, restated.  A policy that ends in logits leaves the choice to
+`collect` and the stored actions' log-probabilities to `RolloutSlots.evaluate` (policy_ops.py).
 """
 import torch
+
+from .policy_ops import action_log_probs, pick_actions
 
 
 def get_leaf_nodes(observation, internal_node_holder, leaf_node_holder):
@@ -18,6 +21,14 @@ def get_leaf_nodes(observation, internal_node_holder, leaf_node_holder):
     unify_obs = observation.reshape((observation.shape[0], -1, 9))
     leaf_nodes = unify_obs[:, internal_node_holder:internal_node_holder + leaf_node_holder, :]
     return unify_obs, leaf_nodes
+
+
+def leaf_mask(all_nodes, leaf_node_holder):
+    """[N,I+L+1,9] -> [N,L] (a view): column 8 of the leaf nodes, not zero where there is one."""
+    total = all_nodes.shape[1]
+    if not 0 < leaf_node_holder < total:
+        raise ValueError("%d leaves do not fit observations of %d nodes" % (leaf_node_holder, total))
+    return all_nodes[:, total - 1 - leaf_node_holder:total - 1, 8]
 
 
 class RolloutSlots(object):
@@ -72,6 +83,17 @@ class RolloutSlots(object):
         for step in reversed(range(self.rewards.size(0))):
             self.returns[step] = self.returns[step + 1] * self.gamma * self.masks[step + 1] + self.rewards[step]
 
+    def evaluate(self, logits, top=0):
+        """What an update needs of the stored steps: `action_log_probs` of the stored actions under `logits` [T * N, L] (or
+        [T, N, L]), computed by the caller's policy from `obs[:-1]`, over each observation's valid leaves.  Log-probabilities
+        come as [T * N, 1], the entropy as [T * N]; differentiable with respect to `logits`."""
+        rows = self.num_steps * self.actions.shape[1]
+        logits = logits.reshape(-1, logits.shape[-1])
+        if logits.shape[0] != rows:
+            raise ValueError("evaluate: logits of %d rows for %d stored actions" % (logits.shape[0], rows))
+        mask = leaf_mask(self.obs[:-1].view(rows, -1, 9), logits.shape[1])
+        return action_log_probs(logits, self.actions.view(rows, 1), mask=mask, top=top)
+
     def gather(self, group=None):
         """All ranks' shards as storage-shaped tensors (env axis = dim 1), over RCCL/xGMI."""
         from .sharding import gather_rollout
@@ -85,11 +107,13 @@ class RolloutSlots(object):
 DeviceRollout = RolloutSlots  # round-1 name
 
 
-def collect(envs, policy, rollout):
+def collect(envs, policy, rollout, sample=True):
     """train_tools.py:63-70 without host round trips and without copy kernels: per step the policy and ONE
-    transition launch.  `policy(all_nodes [N,I+L+1,9]) -> (log_prob [N,1], leaf_index int64 [N,1])`; `envs` is a
-    PctVecEnv; if its current observation is not the rollout's current slot yet, the slot is seeded from it.
-    Returns the last observation view."""
+    transition launch.  `policy(all_nodes [N,I+L+1,9])` gives `(log_prob [N,1], leaf_index int64 [N,1])`, or logits [N,L]
+    alone: then the choice is made here among the observation's valid leaves (`pick_actions`, with Gumbel noise from torch's
+    generator if `sample`, else the best) and written straight into the rollout's slots.  `envs` is a PctVecEnv; if its
+    current observation is not the rollout's current slot yet, the slot is seeded from it.  Returns the last observation
+    view."""
     cur = envs.current_obs()
     slot = rollout.obs[rollout.step]
     if cur.data_ptr() != slot.data_ptr():
@@ -98,7 +122,16 @@ def collect(envs, policy, rollout):
         slot.copy_(cur.view_as(slot))
     all_nodes = slot
     for _ in range(rollout.num_steps):
+        nodes = all_nodes.view(all_nodes.shape[0], -1, 9)  # tools.py:70-73 unify_obs
         with torch.no_grad():
-            log_prob, idx = policy(all_nodes.view(all_nodes.shape[0], -1, 9))  # tools.py:70-73 unify_obs
+            said = policy(nodes)
+        if torch.is_tensor(said):
+            t = rollout.step
+            noise = torch.empty(said.shape, device=said.device).exponential_().log_().neg_() if sample else None
+            idx = pick_actions(said, mask=leaf_mask(nodes, said.shape[1]), noise=noise, actions_out=rollout.actions[t],
+                               log_probs_out=rollout.action_log_probs[t]).actions
+            log_prob = None  # (it stands in its slot already)
+        else:
+            log_prob, idx = said
         all_nodes = rollout.step_env(envs, idx, log_prob)
     return all_nodes

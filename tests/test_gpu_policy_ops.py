@@ -367,6 +367,20 @@ def test_attention_is_repeatable_and_splits_agree():
             _close(got, w, e, "splits")
 
 
+@pytest.mark.parametrize("kind", ["bool", "column", "i32", "f16"])
+def test_key_masks_of_every_type_and_length(kind):
+    for lk in (1, 2, 63, 64, 65, 257, 511, 512, 513):
+        q, k, v, _ = _qkv((7, 2, lk, 1, 1, 8), "f32", lk)
+        mask = _mask(kind, 7, lk, lk)
+        n = torch.randint(0, lk + 2, (7,), generator=_gen(lk))
+        n[1] = lk
+        for lengths in (None, n.cuda()):
+            allowed = (mask != 0).cpu() & (torch.arange(lk)[None] < n[:, None] if lengths is not None else True)
+            out = _pkg().cross_attention(q, k, v, key_mask=mask, key_lengths=lengths)
+            want, bound = ref.attention(q, k, v, allowed, 1 / math.sqrt(8))
+            _close(out, want[0], bound[0], (kind, lk))
+
+
 def test_attention_empty_sizes():
     pk = _pkg()
     for shape in ((0, 3, 4, 1, 1, 16), (2, 0, 4, 1, 1, 16), (2, 3, 0, 2, 1, 16)):
@@ -545,3 +559,85 @@ def test_long_rows_past_two_to_the_32_bytes():
     x[39999, 59999] = 20.0
     o = _pkg().pick_actions(x)
     assert o.actions[39999].item() == 59999 and o.actions[39998].item() == 0
+
+
+def _plain_leaf_policy(w, heads, nodes, i, l):
+    """LeafPolicy from its weights `w` (64 bits, CPU), elementary operations only"""
+    lin = lambda x, name: x @ w[name + ".weight"].T + w[name + ".bias"]
+    mask = nodes[:, :, 8] != 0
+    kind = torch.cat([torch.full((n,), j) for j, n in enumerate((i, l, 1))])
+    x = lin(nodes, "embed") + w["kinds"][kind]
+
+    def attend(q, k, v):
+        split = lambda t: t.reshape(t.shape[0], t.shape[1], heads, -1).transpose(1, 2)
+        q, k, v = split(q), split(k), split(v)
+        s = (q @ k.transpose(2, 3)) / math.sqrt(q.shape[3])
+        p = s.masked_fill(~mask[:, None, None, :], -math.inf).softmax(3)
+        return (p @ v).transpose(1, 2).flatten(2)
+
+    x = x + attend(*lin(x, "node_qkv").chunk(3, 2))
+    leaves = x[:, i:i + l]
+    return lin(torch.tanh(leaves + attend(lin(leaves, "leaf_q"), *lin(x, "leaf_kv").chunk(2, 2))), "score")[:, :, 0]
+
+
+@pytest.mark.parametrize("heads", [1, 2])
+def test_leaf_policy_and_its_gradients(heads):
+    pk = _pkg()
+    torch.manual_seed(3)
+    i, l, n = 20, 9, 5
+    net = pk.LeafPolicy(i, l, width=32, heads=heads, device="cuda")
+    nodes = torch.rand(n, i + l + 1, 9, generator=_gen(1))
+    nodes[:, :, 8] = (torch.rand(n, i + l + 1, generator=_gen(2)) < 0.5).float()
+    nodes[:, -1, 8] = 1.0
+    d = torch.randn(n, l, generator=_gen(3))
+    logits = net(nodes.cuda())
+    grads = torch.autograd.grad(logits, list(net.parameters()), d.cuda())
+    w = {k: p.detach().double().cpu().requires_grad_(True) for k, p in net.named_parameters()}
+    want = _plain_leaf_policy(w, heads, nodes.double(), i, l)
+    wg = torch.autograd.grad(want, list(w.values()), d.double())
+    # five products of at most 32 terms, two softmaxes of at most 30 and a sum over 150 nodes, 2^-24 each of values below 2^3
+    tol = (5 * 32 + 2 * 30 + 150) * 2.0 ** -24 * 8
+    assert (logits.detach().double().cpu() - want).abs().max() < tol
+    for a, b, name in zip(grads, wg, w):
+        assert (a.double().cpu() - b).abs().max() <= tol * max(1.0, b.abs().max().item()), name
+
+
+def test_collect_with_logits_and_evaluate():
+    """the rollout path: a policy of logits, the choice made by collect, the update's log-probabilities and gradients"""
+    pk = _pkg()
+    items = [(a, b, c) for a in range(1, 6) for b in range(1, 6) for c in range(1, 6)]
+    make = lambda: pk.PctVecEnv(24, setting=2, item_set=items, internal_node_holder=80, leaf_node_holder=50, seed=9)
+    torch.manual_seed(5)
+    net = pk.LeafPolicy(80, 50, width=32, device="cuda")
+    for sample in (True, False):
+        env = make()
+        env.reset()
+        slots = pk.RolloutSlots(6, 24, (131 * 9,), 1.0, "cuda")
+        torch.manual_seed(6)
+        last = pk.collect(env, net, slots, sample=sample)
+        assert last.data_ptr() == slots.obs[6].data_ptr()
+        env.unbind_rollout_slot()
+        # the same steps by hand
+        torch.manual_seed(6)
+        env = make()
+        obs = env.reset()
+        for t in range(6):
+            nodes, leaves = pk.get_leaf_nodes(obs, 80, 50)
+            assert torch.equal(nodes.reshape(24, -1), slots.obs[t])
+            with torch.no_grad():
+                x = net(nodes)
+            noise = torch.empty(24, 50, device="cuda").exponential_().log_().neg_() if sample else 0.0
+            best = (x + noise).masked_fill(leaves[:, :, 8] == 0, -math.inf).argmax(1, keepdim=True)
+            assert torch.equal(best, slots.actions[t])
+            obs = env.step(best)[0]
+        res = slots.evaluate(net(slots.obs[:-1].view(-1, 131, 9)))
+        # (the same rows in a batch of 144: products of 32 and sums of 50 terms in another order)
+        assert (res.log_probs.detach().view(6, 24, 1) - slots.action_log_probs).abs().max() < 1e-4
+        logits = net(slots.obs[:-1].view(-1, 131, 9)).detach().view(6, 24, 50).requires_grad_(True)
+        res = slots.evaluate(logits, top=3)
+        g, = torch.autograd.grad(res.log_probs.sum() + 0.1 * res.entropy.sum(), [logits])
+        mask = pk.leaf_mask(slots.obs[:-1].view(-1, 131, 9), 50)
+        allowed, empty, logp, p, h = ref.choice(logits.view(-1, 50), mask)
+        assert not empty.any() and (res.top_actions[:, 0].cpu() == logits.detach().view(-1, 50).cpu().masked_fill(~allowed, -math.inf).argmax(1)).all()
+        want, size = ref.choice_gradient(allowed, p, logp, h, [(slots.actions.view(-1, 1), torch.ones(144, 1))], torch.full((144,), 0.1))
+        _close(g.view(-1, 50), want, 1e-5 * (size + p), "gradient")

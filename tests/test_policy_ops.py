@@ -146,3 +146,26 @@ def test_workspace_of_the_longest_rows():
     for choices in (2 ** 31 - 1, 2 ** 31 - 100, 2 ** 31 - 4096, 2 ** 30):
         assert L.pct_choice_workspace(1, choices, 0) == 64 * 32
         assert L.pct_choice_workspace(2 ** 31 - 1, choices, 0) == 0
+
+
+def test_leaf_mask_and_its_callers_refusals():
+    pk = _pkg()
+    nodes = torch.arange(2 * 14 * 9, dtype=torch.float32).view(2, 14, 9)
+    m = pk.leaf_mask(nodes, 5)
+    assert torch.equal(m, nodes[:, 8:13, 8]) and m.data_ptr() == nodes[:, 8:, 8].data_ptr()
+    for bad in (0, 14, 20, -1):
+        with pytest.raises(ValueError):
+            pk.leaf_mask(nodes, bad)
+    r = pk.RolloutSlots(3, 2, (14, 9), 1.0, "cpu")
+    with pytest.raises(ValueError):
+        r.evaluate(torch.zeros(5, 5))
+    with pytest.raises(pk.PctEnvError, match="no CPU path"):
+        r.evaluate(torch.zeros(3, 2, 5))
+    for width, heads in ((60, 1), (64, 3), (136, 1), (32, 8)):
+        with pytest.raises(ValueError):
+            pk.LeafPolicy(8, 5, width=width, heads=heads)
+    net = pk.LeafPolicy(8, 5, width=16)
+    with pytest.raises(ValueError):
+        net(torch.zeros(2, 13, 9))
+    with pytest.raises(pk.PctEnvError, match="no CPU path"):
+        net(nodes)
