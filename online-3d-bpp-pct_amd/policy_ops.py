@@ -162,9 +162,10 @@ def _check_logits(name, logits):
         raise ValueError("%s: rows and choices must be below 2^31" % name)
 
 
-def _out(name, t, shape, dtype, dev):
+def _out(name, t, shape, dtype, x):
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
+        return x.new_empty(shape, dtype=dtype)  # (a microsecond less than torch.empty with a device)
+    dev = x.device
     if t.dtype != dtype or t.device != dev or t.numel() != math.prod(shape) or not t.is_contiguous():
         raise ValueError("%s must be a contiguous %s tensor of %s on %s" % (name, dtype, tuple(shape), dev))
     return t
@@ -188,13 +189,13 @@ def pick_actions(logits, mask=None, noise=None, actions_out=None, log_probs_out=
             raise ValueError("pick_actions: noise must be float32 of the logits' shape")
         noise = _rows_of(noise)
     dev = _on_gpu("pick_actions", logits, mask, noise, actions_out, log_probs_out)
-    actions = _out("actions_out", actions_out, (n, 1), torch.int64, dev)
-    log_probs = _out("log_probs_out", log_probs_out, (n, 1), torch.float32, dev)
-    entropy = torch.empty(n, dtype=torch.float32, device=dev)
+    actions = _out("actions_out", actions_out, (n, 1), torch.int64, x)
+    log_probs = _out("log_probs_out", log_probs_out, (n, 1), torch.float32, x)
+    entropy = x.new_empty(n, dtype=torch.float32)
     if n:
         L = _library()
         ws_bytes = L.pct_choice_workspace(n, v, 0)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
         c = _Choice(_CHOICE_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask), m_row, m_col, m_type, 0, None,
                     0, 0, _ptr(noise), noise.stride(0) if noise is not None else 0, actions.data_ptr(), log_probs.data_ptr(),
                     entropy.data_ptr(), None, None, None, _ptr(ws), ws_bytes)
@@ -206,15 +207,15 @@ def _log_probs_forward(x, given, mask, top, want_stats):
     n, v = x.shape
     dev = x.device
     g = given.shape[1]
-    log_probs = torch.empty(n, g, dtype=torch.float32, device=dev)
-    entropy = torch.empty(n, dtype=torch.float32, device=dev)
-    top_log_probs = torch.empty(n, top, dtype=torch.float32, device=dev) if top else None
-    top_actions = torch.empty(n, top, dtype=torch.int64, device=dev) if top else None
-    stats = torch.empty(n, 4, dtype=torch.float32, device=dev) if want_stats else None
+    log_probs = x.new_empty((n, g), dtype=torch.float32)
+    entropy = x.new_empty(n, dtype=torch.float32)
+    top_log_probs = x.new_empty((n, top), dtype=torch.float32) if top else None
+    top_actions = x.new_empty((n, top), dtype=torch.int64) if top else None
+    stats = x.new_empty((n, 4), dtype=torch.float32) if want_stats else None
     if n:
         L = _library()
         ws_bytes = L.pct_choice_workspace(n, v, top)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
         c = _Choice(_CHOICE_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask[0]), mask[1], mask[2], mask[3],
                     g, given.data_ptr(), top, 0, None, 0, None, log_probs.data_ptr(), entropy.data_ptr(), _ptr(top_log_probs),
                     _ptr(top_actions), _ptr(stats), _ptr(ws), ws_bytes)
@@ -240,7 +241,7 @@ class _LogProbs(torch.autograd.Function):
     def backward(ctx, d_log_probs, d_entropy, d_top=None, _=None):
         x, given, mask, top_actions, stats = ctx.saved_tensors
         n, v = x.shape
-        dx = torch.empty(n, v, dtype=x.dtype, device=x.device)
+        dx = x.new_empty((n, v))
         if n:
             d_log_probs, d_entropy, d_top = (None if t is None else t.contiguous() for t in (d_log_probs, d_entropy, d_top))
             m_row, m_col, m_type = ctx.mask_args
@@ -314,11 +315,11 @@ def _attention_struct(q, k, v, mask, lengths, scale, out, stats, key_list):
                       0 if lengths is None else lengths.element_size(), _ptr(lengths), scale, 0, out.data_ptr(), _ptr(stats), _ptr(key_list))
 
 
-def _workspace(L, a, backward, dev):
+def _workspace(L, a, backward, like):
     a.workspace_bytes = L.pct_attend_workspace(ctypes.addressof(a), backward)
     if not a.workspace_bytes:
         return None
-    ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=dev)
+    ws = like.new_empty(a.workspace_bytes, dtype=torch.uint8)
     a.workspace = ws.data_ptr()
     return ws
 
@@ -326,13 +327,13 @@ def _workspace(L, a, backward, dev):
 def _attend_forward(q, k, v, mask, lengths, scale, want_stats):
     b, lq, h, d = q.shape
     dev, hk = q.device, k.shape[2]
-    out = torch.empty(b, lq, h, d, dtype=q.dtype, device=dev)
-    stats = torch.empty(b * lq * h * 2, dtype=torch.float32, device=dev) if want_stats else None
-    key_list = torch.empty(b, k.shape[1] + 1, dtype=torch.int32, device=dev) if mask[0] is not None else None
+    out = q.new_empty((b, lq, h, d))
+    stats = q.new_empty(b * lq * h * 2, dtype=torch.float32) if want_stats else None
+    key_list = q.new_empty((b, k.shape[1] + 1), dtype=torch.int32) if mask[0] is not None else None
     if b and lq:
         L = _library()
         a = _attention_struct(q, k, v, mask, lengths, scale, out, stats, key_list)
-        ws = _workspace(L, a, 0, dev)  # noqa: F841  (held until the call has been enqueued)
+        ws = _workspace(L, a, 0, q)  # noqa: F841  (held until the call has been enqueued)
         _call(L.pct_attend, a, dev)
     return out, stats, key_list
 
@@ -353,15 +354,13 @@ class _CrossAttention(torch.autograd.Function):
         q, k, v, lengths, out, stats, key_list = ctx.saved_tensors
         d_out = _attention_rows(d_out)
         dev = q.device
-        d_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        d_k = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        d_v = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        d_q, d_k, d_v = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         if q.shape[0]:
             L = _library()
             a = _attention_struct(q, k, v, (key_list, 0, 0, 4), lengths, ctx.scale, out, stats, key_list)
             a.d_out, a.d_out_stride = d_out.data_ptr(), _strides(d_out)
             a.d_q, a.d_k, a.d_v = d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr()
-            ws = _workspace(L, a, 1, dev)  # noqa: F841
+            ws = _workspace(L, a, 1, q)  # noqa: F841
             _call(L.pct_attend_backward, a, dev)
         return d_q, d_k, d_v, None, None, None, None, None, None
 
