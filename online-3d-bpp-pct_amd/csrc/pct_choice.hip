@@ -175,6 +175,27 @@ __global__ __launch_bounds__(TEAM == 1 ? 256 : 64 * TEAM) void pct_choice_kernel
   best.start();
   float score = 0.f;
   int pick = -1;
+  // 16-bit rows: the next step's logits (and bytes of the mask) are on their way while this step's are worked on.  8192 x 65536
+  // bfloat16: 265 us without, 240 so (4.5 TB/s); no gain where a list is kept (the sorts hide it) or for float32 (twice the bytes to
+  // the same work).
+  constexpr bool AHEAD = VEC == 8 && sizeof(T) == 2 && MODE != LOGP_TOP;
+  // (the mask's only without noise, whose loads take the registers: 4000 x 30000 98 -> 87 us, but 5000 x 20000 with noise 133 -> 147)
+  constexpr bool MASK_AHEAD = AHEAD && MASK == M_BYTES && MODE == LOGP;
+  using Raw = typename Vec8<T>::raw;
+  Raw ahead[AHEAD ? U : 1];
+  Bytes8 ahead_mask[MASK_AHEAD ? U : 1];
+  auto fetch = [&](int64_t base) {
+    if constexpr (AHEAD) {
+      const int64_t i0 = base + (int64_t)(TEAM == 1 ? lane : (int)threadIdx.x) * VEC;
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (i0 + u * STEP + VEC <= c1) {
+          ahead[u] = *(const Raw*)(x + i0 + u * STEP);
+          if constexpr (MASK_AHEAD) ahead_mask[u] = *(const Bytes8*)((const uint8_t*)p.mask.p + (int64_t)row * p.mask.row + i0 + u * STEP);
+        }
+    }
+  };
+  fetch(c0);
   // (the loop runs the same number of times in every lane: the top list needs whole wavefronts)
 #pragma unroll 1
   for (int64_t base = c0; base < c1; base += (int64_t)STEP * U) {
@@ -187,9 +208,12 @@ __global__ __launch_bounds__(TEAM == 1 ? 256 : 64 * TEAM) void pct_choice_kernel
       if constexpr (VEC == 8) {
         if (i + VEC <= c1) {
           whole = true;
-          load8(x + i, v[u]);
+          if constexpr (AHEAD) unpack8<T>(ahead[u], v[u]);
+          else load8(x + i, v[u]);
           if (MASK == M_BYTES) {
-            const Bytes8 b = *(const Bytes8*)((const uint8_t*)p.mask.p + (int64_t)row * p.mask.row + i);
+            Bytes8 b;
+            if constexpr (MASK_AHEAD) b = ahead_mask[u];
+            else b = *(const Bytes8*)((const uint8_t*)p.mask.p + (int64_t)row * p.mask.row + i);
 #pragma unroll
             for (int e = 0; e < VEC; e++) v[u][e] = (b.w[e / 4] & (0xffu << (8 * (e % 4)))) ? v[u][e] : -INFINITY;
           } else if (MASK == M_ANY) {
@@ -209,6 +233,7 @@ __global__ __launch_bounds__(TEAM == 1 ? 256 : 64 * TEAM) void pct_choice_kernel
         }
       }
     }
+    fetch(base + (int64_t)STEP * U);
     float top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; u++)

@@ -26,8 +26,7 @@ template <typename T> struct Vec8 { using raw = Half8; };
 template <> struct Vec8<float> { using raw = Float8; };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&o)[8]) {
-  typename Vec8<T>::raw r = *(const typename Vec8<T>::raw*)p;
+__device__ __forceinline__ void unpack8(const typename Vec8<T>::raw& r, float (&o)[8]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < 8; i++) o[i] = __uint_as_float(r.w[i]);
@@ -44,6 +43,9 @@ __device__ __forceinline__ void load8(const T* p, float (&o)[8]) {
     }
   }
 }
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&o)[8]) { unpack8<T>(*(const typename Vec8<T>::raw*)p, o); }
 
 // two values rounded to nearest even and packed
 template <typename T>
