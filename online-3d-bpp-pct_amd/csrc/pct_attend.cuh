@@ -299,6 +299,10 @@ struct Power {
 };
 
 // ------------------------------------------------------------------------------------------------------------- forward
+// Measured: 4 x 16 heads x 2048 x 4096 x 128 bfloat16 331 us, 830 TFLOP/s (a library product of 8192^3: 1134) -- two wavefronts to a
+// SIMD that wait for their own products and exponentials in turn; 2048 x 4 x 200 x 401 x 32 with 29 % of the keys 128 us, where
+// vector instructions are 59 % busy and HBM moves 2.6 TB/s; 4096 x 131 x 131 x 64 float32 163 us, its matrix instructions at 35 % of
+// their peak; single queries, 16 x 8 heads x 16384 x 128, 161 us, 5 TB/s.
 template <typename T, int DP, int MAXW, int R>
 __global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
   using L = Tile<T, DP, R>;
@@ -520,6 +524,8 @@ __device__ __forceinline__ float p_value(float s, float c, float2 t) {
 // D_r = dO_r . O_r, where O_r has been rounded to the tensors' type: over many keys that error vanishes beside dP, over few it
 // would not, so where all keys fit one tile of 16-bit elements D is summed from P dP itself.  So is that of a lone key, in every
 // type: its dS is then exactly 0.
+// Measured: 4 x 16 x 2048 x 4096 x 128 bfloat16 460 us, 895 TFLOP/s over three products; 2048 x 4 x 200 x 401 x 32 188 us; 4096 x 131 x
+// 131 x 64 float32 252 us, 34 % of the matrix peak at two wavefronts to a SIMD (more would spill).
 template <typename T, int DP, int MAXW>
 __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p) {
   using L = Tile<T, DP>;
@@ -673,6 +679,9 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p
 }
 
 // --------------------------------------------------------------------------------------------------------------- dk, dv
+// The same tiles with the sides changed: keys stay, q and d_out pass.  S and dP are computed a second time, which costs two products
+// of seven and needs neither atomics nor dS in memory.  Measured: 4 x 16 x 2048 x 4096 x 128 bfloat16 611 us, 900 TFLOP/s over four
+// products; 2048 x 4 x 200 x 401 x 32 174 us; 4096 x 131 x 131 x 64 float32 250 us, 46 % of the matrix peak.
 template <typename T, int DP, int MAXW>
 __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams p) {
   using L = Tile<T, DP>;
@@ -821,6 +830,7 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams 
 }
 
 // clears dk and dv of the keys that are not allowed, all heads of one at a time: a workgroup to a batch, 16 bytes to a thread
+// (2048 x 401 keys of 4 x 32, 71 % of them: 41 us, 7 TB/s)
 template <typename T>
 __global__ __launch_bounds__(256) void pct_attend_clear_kernel(AttendParams p, int chunks, int b0) {
   const int b = b0 + blockIdx.x, n = allowed_keys(p, b);

