@@ -7,10 +7,11 @@
 // (profiles/r04_lstsq_ondomain.txt).  This file is the strict alternative: the path dgelsd takes for these systems
 // (M = k (k - 1) / 2 + 1 rows, k <= 16 columns, one right-hand side), operation for operation --
 //   dgeqr2, dorm2r (Q^T b), dgebd2, dorm2r, dlalsd (scale, dlasdq = dbdsqr with vectors + sort, rank cut, V (.)), dorml2 --
-// with the arithmetic of the BLAS kernels OpenBLAS 0.3.29 dispatches to on AVX-512 hosts (NumPy 2.2.6's bundled library in
-// the build container; PCT_LSTSQ_GELSD) or on AVX2 hosts, AMD Zen included (its "Haswell" kernel set; PCT_LSTSQ_GELSD_AVX2 --
-// dgemv 'N', daxpy and the dgemm kernel differ): which products are fused, how many lanes a sum is split over, and dnrm2's
-// 80-bit x87 accumulation, emulated here with 64-bit integer mantissas.  Plain IEEE double operations otherwise (the library is built with
+// with the arithmetic that the BLAS of NumPy 2.2.6 (OpenBLAS 0.3.29) shows in its results on AVX-512 hosts (PCT_LSTSQ_GELSD) or on
+// AVX2 hosts, AMD Zen included (its "Haswell" kernel set; PCT_LSTSQ_GELSD_AVX2 -- dgemv 'N', dger and dgemm differ): which products
+// are fused, in which tree a sum is added, and the 64 bits that dnrm2's squares and sums are rounded to, emulated here with integer
+// mantissas.  tests/golden/derive_blas_orders.py finds that tree of every sum by calls alone (profiles/blas_orders_skylakex.txt,
+// _haswell.txt); the formulas here are the ones it prints.  Plain IEEE double operations otherwise (this file is compiled with
 // -ffp-contract=off; fma() is v_fma_f64 / the C fma, division and sqrt are correctly rounded on both sides).
 // The routines work on a workspace in LDS (no private arrays, no calls) and are written for a GROUP of G lanes of one wavefront
 // per system (round 5; G = 1: one lane, which is also how tests/host compiles them for the CPU, where tests/test_stab_host.py
@@ -59,7 +60,7 @@ namespace gelsd {
 // the lanes that share one system: lane gl of G (G = 1: one lane does everything)
 struct Grp { int gl, G; };
 
-// ---- 80-bit extended precision (x87, round to nearest even, 64-bit mantissa), non-negative values only -----------------------
+// ---- extended precision: a 64-bit mantissa, rounded to nearest even, non-negative values only ---------------------------------
 // value = m * 2^e with 2^63 <= m < 2^64, or m == 0
 struct Ext { uint64_t m; int e; };
 
@@ -90,7 +91,7 @@ PCT_GD Ext ext_round(uint64_t hi, uint64_t lo, bool sticky, int e) {
   }
   return r;
 }
-// fld + fmul st(0): the square of a double, rounded to 64 bits
+// the square of a double, rounded to 64 bits
 PCT_GD Ext ext_square(double v) {
   Ext z;
   z.m = 0; z.e = 0;
@@ -121,7 +122,7 @@ PCT_GD Ext ext_square(double v) {
   }
   return ext_round(hi, lo, false, e);
 }
-// faddp of two non-negative values
+// the sum of two, rounded to 64 bits
 PCT_GD Ext ext_add(Ext x, Ext y) {
   if (y.m == 0) return x;
   if (x.m == 0) return y;
@@ -145,7 +146,7 @@ PCT_GD Ext ext_add(Ext x, Ext y) {
   }
   return ext_round(hi, lo, sticky, e);
 }
-// fsqrt, then fstp qword: the square root rounded to 64 bits, then to a double
+// the square root, rounded to 64 bits and then to a double (one rounding gives other results: derive_blas_orders.py)
 PCT_GD double ext_sqrt_to_double(Ext x) {
   if (x.m == 0) return 0.0;
   // N = x.m << 64 (exponent e - 64) or x.m << 63 (exponent e - 63), whichever exponent is even; root = isqrt(N), 2^63 <= root
@@ -238,17 +239,17 @@ PCT_GD double ext_sqrt_to_double(Ext x) {
   return cv.d;
 }
 
-// ---- BLAS, as OpenBLAS' SkylakeX kernel set computes it (kernel/x86_64: nrm2.S, dgemv_t_4.c + Haswell microkernels,
-// dgemv_n_4.c + SkylakeX microkernel, ger.c -> daxpy, drot + SkylakeX microkernel) ------------------------------------------
+// ---- BLAS: the arithmetic that the outputs determine ------------------------------------------------------------------------
 // dnrm2: accumulators A..D over the leading blocks of eight (element i into accumulator i mod 4), the tail into A,
-// ((C + A) + B) + D, fsqrt, one rounding to double.  (Every lane of a group runs it: the loads are LDS broadcasts, eight in
-// flight at a time; the accumulation is the serial chain it is on the FPU.)
+// ((C + A) + B) + D, every square and sum rounded to 64 bits, the root to 64 and then to a double: of the 490 ways to sum that
+// derive_blas_orders.py tries, the only one whose results near rounding boundaries are the library's.  (Every lane of a group runs
+// it: the loads are LDS broadcasts, eight in flight at a time; the accumulation is a serial chain.)
 // The same value WITHOUT the integer emulation, for up to eight elements, when a certificate holds (round 6).  dnrm2 returns
-// round53(round64(sqrt(S))) with S the x87 sum: every square and every partial sum rounded to 64 bits, so S = T (1 + e),
+// round53(round64(sqrt(S))) with S the 64-bit sum: every square and every partial sum rounded to 64 bits, so S = T (1 + e),
 // |e| <= (n + 4) 2^-64 <= 12 * 2^-64 for the exact sum of squares T (all terms non-negative), and round64(sqrt(S)) lies within
 // 2^-61 sqrt(T) of sqrt(T).  Here T is accumulated as a double-double (squares exact by FMA, two-sum additions: relative error
 // < 2^-100), its root as s + c with s = sqrt(T_hi) and c = (T_hi - s^2 + T_lo) / 2s (the residual of a square root is exact in one
-// FMA; error of s + c below 2^-100 sqrt(T)), and R = fl(s + c) is the correct rounding of that pair.  R is ALSO the x87 value
+// FMA; error of s + c below 2^-100 sqrt(T)), and R = fl(s + c) is the correct rounding of that pair.  R is ALSO that value
 // whenever s + c keeps a distance of more than 2^-60 R from the nearest rounding boundary (the midpoint of two neighbouring
 // doubles: half an ulp from R, a quarter below a power of two) -- tested with a margin of 2 % of half an ulp = 2^-59.6 R.  Otherwise
 // (2 % of the calls), or when a square could leave the double range, the caller runs the emulation.  Checked against it on
@@ -285,7 +286,7 @@ PCT_GD double dnrm2_ext(int n, const double* x, int incx);
 PCT_GD double dnrm2(int n, const double* x, int incx) {
   if (n <= 0) return 0.0;
 #if !defined(PCT_GELSD_NO_NRM2_SHORTCUT)
-  // One element: fsqrt(round64(x^2)) = |x| (1 + d) with |d| < 2^-64, |x| a 53-bit number: the 64-bit rounding of the root and the
+  // One element: round64(sqrt(round64(x^2))) = |x| (1 + d) with |d| < 2^-64, |x| a 53-bit number: the 64-bit rounding of the root and the
   // store to double both return |x| (checked against the long chain: tests/test_stab_host.py).  Three of the six non-trivial
   // reflectors of a three-supporter system have such a one-element tail.
   if (n == 1) return fabs(x[0]);
@@ -337,7 +338,7 @@ PCT_GD double dnrm2_ext(int n, const double* x, int incx) {
 }
 // dnrm2 by the group, for vectors long enough to pay two hand-overs through LDS: the squares an element per lane, then the four
 // accumulator chains (A: elements 0, 4, 8 ... of the leading blocks of eight and then the tail, in order; B, C, D: elements 1, 2, 3
-// mod 4 of the blocks) a chain per lane -- every chain the serial x87 sum it is on the FPU -- and ((C + A) + B) + D, the root and the
+// mod 4 of the blocks) a chain per lane -- every chain a serial sum -- and ((C + A) + B) + D, the root and the
 // rounding in every lane.  The value is dnrm2's bit for bit: the same additions in the same order within each accumulator.
 // scratch: 2 n + 8 doubles nobody else uses meanwhile (split_t: the V^T region, idle until dbdsqr).
 #ifndef PCT_GELSD_COOP_NRM2_MIN
@@ -404,11 +405,11 @@ PCT_GD double dnrm2_g(Grp g, int n, const double* x, int incx, double* scratch) 
 PCT_GD void dscal(Grp g, int n, double alpha, double* x, int incx) {
   for (int i = g.gl; i < n; i += g.G) x[i * incx] = alpha * x[i * incx];
 }
-// One column of y = A^T x (alpha = 1, beta = 0), column j of n (c points at it): rows in groups of four -- by the 4x4 kernel
-// (AVX2 FMA, four lanes, (l0 + l2) + (l1 + l3)) for the columns of the leading groups of four, then two columns by the 4x2
-// kernel (SSE2, two lanes, products and sums rounded separately, l0 + l1), then one by the 4x1 kernel (SSE2, (r0 + r2) +
-// (r1 + r3)) -- and the m mod 4 tail rows: t = a1 x1; fma(a0, x0, t); fma(a2, x2, t); y + t.  Which kernel a column meets
-// depends on its POSITION j among the n columns of the call.
+// One column of y = A^T x (alpha = 1, beta = 0), column j of n (c points at it).  The rows but the last m mod 4: a column of the
+// leading groups of four is summed in four chains of fused products (row mod 4), (l0 + l2) + (l1 + l3); of the columns left a pair
+// in two chains of rounded products, l0 + l1, and the last odd one in four chains of rounded products, (l0 + l2) + (l1 + l3).  The
+// last rows: t = a1 x1; fma(a0, x0, t); fma(a2, x2, t); y + t (a lone one is fused into y).  How a column is summed depends on its
+// POSITION j among the n columns of the call.
 PCT_GD double dgemv_t_col(int m, int n, int j, const double* c, const double* x, int incx) {
   const int m2 = m & ~3, m3 = m & 3, n4 = n & ~3;
   double yj = 0.0;
@@ -452,20 +453,20 @@ PCT_GD double dgemv_t_col(int m, int n, int j, const double* c, const double* x,
 }
 // One row of y = A x (alpha = 1, beta = 0), row i of m, with a STRIDED x (dlarf from the right in dgebd2: x is a row of A):
 // rows in groups of four -- columns in groups of four (t = a1 x1; fma a0 x0; fma a2 x2; fma a3 x3; y = fma(1, t, y)), the
-// rest one by one, y + a x rounded separately -- and the tail rows: t = fma(a, x, t) over all columns.  avx2: the Haswell
-// kernel set instead
+// rest one by one, y + a x rounded separately -- and the tail rows: t = fma(a, x, t) over all columns.  avx2: the sums of the
+// Haswell kernel set instead
 PCT_GD double dgemv_n_row(int m, int n, int i, const double* a, int lda, const double* x, int incx, bool avx2) {
   const int m2 = m & ~3, n4 = n & ~3;
   if (i < m2) {
     double yi = 0.0;
     for (int j = 0; j < n4; j += 4) {
       double t;
-      if (avx2) {  // Haswell microkernel: two FMA chains, (a0 x0 + a2 x2) + (a1 x1 + a3 x3)
+      if (avx2) {  // two fused chains, (a0 x0, a2 x2) + (a1 x1, a3 x3)
         double t4 = a[i + j * lda] * x[j * incx], t5 = a[i + (j + 1) * lda] * x[(j + 1) * incx];
         t4 = fma(a[i + (j + 2) * lda], x[(j + 2) * incx], t4);
         t5 = fma(a[i + (j + 3) * lda], x[(j + 3) * incx], t5);
         t = t4 + t5;
-      } else {     // SkylakeX microkernel: one chain starting from a1 x1
+      } else {     // one chain starting from a1 x1
         t = a[i + (j + 1) * lda] * x[(j + 1) * incx];
         t = fma(a[i + j * lda], x[j * incx], t);
         t = fma(a[i + (j + 2) * lda], x[(j + 2) * incx], t);
@@ -476,16 +477,16 @@ PCT_GD double dgemv_n_row(int m, int n, int i, const double* a, int lda, const d
     for (int j = n4; j < n; j++) yi = yi + a[i + j * lda] * (x[j * incx] * 1.0);
     return yi;
   }
-  // the C tail: one FMA chain (SkylakeX build) / products and sums rounded separately (Haswell build)
+  // the last rows: one chain of fused products / products and sums rounded separately
   double t = 0.0;
   for (int j = 0; j < n; j++) t = avx2 ? t + a[i + j * lda] * x[j * incx] : fma(a[i + j * lda], x[j * incx], t);
   return avx2 ? 0.0 + 1.0 * t : fma(1.0, t, 0.0);
 }
-// dger's element: A += alpha x y^T is, per column, t = alpha y_j and a_ij = fma(t, x_i, a_ij) (daxpy; Haswell daxpy: blocks of
-// sixteen through the FMA microkernel, the rest multiply and add rounded separately -- `fused` says which)
+// dger's element: A += alpha x y^T is, per column, t = alpha y_j and a_ij = fma(t, x_i, a_ij) (Haswell: fused in the leading blocks
+// of sixteen rows, rounded before the addition in the rest -- `fused` says which)
 PCT_GD double dger_elem(double t, double xi, double aij, bool fused) { return fused ? fma(t, xi, aij) : aij + t * xi; }
 
-// ---- LAPACK 3.11 (compiled Fortran: plain double arithmetic in program order) ----------------------------------------------
+// ---- LAPACK 3.11 (the published Fortran: plain double arithmetic in program order) ----------------------------------------------
 constexpr double EPS = 1.1102230246251565e-16;      // dlamch('E')
 constexpr double SAFMIN = 2.2250738585072014e-308;  // dlamch('S')
 PCT_GD double sgn(double a, double b) { return copysign(fabs(a), b); }
@@ -1325,10 +1326,9 @@ PCT_GD bool split_t(Grp g, double* ws, int k, const double* in, double s0, doubl
   const double tol = rcond * fabs(d[imax]);
   for (int i = 0; i < n; i++)
     if (d[i] > 0.0 && d[i] > tol / ILL_BAND && d[i] < tol * ILL_BAND) ill = true;
-  // b(i) = 0 below the cut, else dlascl(d(i) -> 1) of the one element; then dgemm('T', 'N', n, 1, n): the packed kernel, acc =
-  // fma(vt(k, i), b(k), acc) in k order (Haswell kernel: rows in groups of four with four accumulators over the leading blocks
-  // of eight k, the tail into the first, (q0 + q1) + (q2 + q3); its n mod 4 last rows, like every row of the SkylakeX kernel, one
-  // chain); a row per lane
+  // b(i) = 0 below the cut, else dlascl(d(i) -> 1) of the one element; then dgemm('T', 'N', n, 1, n): acc =
+  // fma(vt(k, i), b(k), acc) in k order (Haswell: rows in groups of four with four accumulators over the leading blocks of eight k,
+  // the tail into the first, (q0 + q1) + (q2 + q3); its n mod 4 last rows one chain); a row per lane
   {
     const Grp one = {0, 1};
     for (int i = g.gl; i < n; i += g.G) {

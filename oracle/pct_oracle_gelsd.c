@@ -13,28 +13,30 @@
  *               dlasv2 / dlas2 / dlartg / dlasr) + selection sort, rank cut at rcond * max(s), divide, V * (.), unscale
  *            -> dorml2 (P b).
  *
- * The LAPACK layer is compiled Fortran without FMA contraction (plain IEEE double operations in program order).  The
- * BLAS layer is OpenBLAS' hand-written kernels, whose summation orders and fused multiply-adds differ per CPU family
- * (the reference's stability verdicts on tie cases differ between machines for that reason: profiles/r04_lstsq_ondomain.txt).
- * Restated here is the kernel set OpenBLAS dispatches to on AVX-512 hosts ("SkylakeX" -- the build container; it reuses
- * the Haswell dgemv_t / daxpy / dger kernels).  Which order each routine sums in and what it fuses shows in its outputs, pair of
- * terms by pair of terms: tests/golden/check_blas_order.py probes the library and this file so, for both kernel sets:
- *   dnrm2   x87: squares and sums in 80-bit extended precision, four accumulators over blocks of eight
- *           (A: i = 0 mod 4 ... D: i = 3 mod 4), the n mod 8 tail into A, ((C + A) + B) + D, fsqrt, ONE rounding to double
- *   dgemv T rows in groups of four: columns in groups of four by the AVX2 kernel (per column four lanes of FMA chains,
- *           (l0 + l2) + (l1 + l3)), then two columns by an SSE2 kernel (two lanes, multiply and add rounded separately,
- *           l0 + l1), then one column by another SSE2 kernel (lanes (r0, r1) and (r2, r3) of each group of four,
- *           (r0 + r2) + (r1 + r3)); y = fma(alpha, t, y) (4x4 columns with unit increment: y + t * alpha).  The m mod 4
- *           tail rows: t = a1 x1; t = fma(a0, x0, t); t = fma(a2, x2, t); y = y + t   (x pre-multiplied by alpha)
- *   dgemv N rows in groups of four: columns in groups of four (t = a1 x1; fma a0 x0; fma a2 x2; fma a3 x3;
- *           y = fma(alpha, t, y)), then (unit-stride x only) a pair (t = a1 x1; fma a0 x0; y = fma(alpha, t, y)), single
- *           columns y = y + a (x alpha) rounded separately; tail rows: t = fma(a, x, t) over all columns, y = fma(alpha, t, y)
- *   dger    per column: t = alpha y_j;  a_ij = fma(t, x_i, a_ij)
- *   drot    x' = fma(c, x, s y);  y' = fma(c, y, -(s x))
- *   dscal   x' = alpha x           dgemm 'T','N' (n x n by n x 1): the packed kernel, acc = fma(a_k, b_k, acc) in k order
- * Every routine below was checked bit for bit against the library's own routine (tests/golden/check_gelsd_port.py calls
- * them through ctypes on random and on recorded systems); the whole solve is checked against np.linalg.lstsq there and
- * -- build-container independent -- against the committed vectors tests/golden/lstsq_systems.npz (tests/test_gelsd_port.py).
+ * The LAPACK layer behaves as its published Fortran evaluated in program order, every operation rounded to a double.  The BLAS
+ * layer sums in orders of its own, which differ per CPU family (the reference's stability verdicts on tie cases differ between
+ * machines for that reason: profiles/r04_lstsq_ondomain.txt).  What each routine returns determines its arithmetic:
+ * tests/golden/derive_blas_orders.py finds, by calls alone, the tree in which every sum adds its products and which of them are
+ * fused, and compares it with this file; so it does for both kernel sets ("SkylakeX": what the library runs on AVX-512 hosts,
+ * "Haswell": on AVX2 hosts; profiles/blas_orders_skylakex.txt, profiles/blas_orders_haswell.txt).  The formulas it finds for
+ * SkylakeX, products in the order in which they are fused, ( ) for a sum of its own:
+ *   dnrm2   squares and sums rounded to 64 bits, four accumulators over the leading blocks of eight (element i into A, B, C, D by
+ *           i mod 4), the n mod 8 last elements into A, ((C + A) + B) + D, the root rounded to 64 bits and then to a double
+ *   dgemv T the rows but the last m mod 4: columns of the leading groups of four by four chains of fused products (i mod 4),
+ *           (l0 + l2) + (l1 + l3); of what is left, a pair of columns by two chains (i mod 2) of rounded products, l0 + l1; the last
+ *           odd column by four chains of rounded products, (l0 + l2) + (l1 + l3).  The last rows are a sum of their own: a1 x1
+ *           rounded, a0 x0 and a2 x2 fused into it; one row alone is fused into the result.  alpha multiplies a block's sum (in the
+ *           groups of four rounded before it is added, else fused) and the last rows' x
+ *   dgemv N rows of the leading groups of four: columns four at a time, a1 x1 rounded, a0 x0, a2 x2, a3 x3 fused into it, alpha
+ *           times that sum fused into the result; then, where x has unit stride, a pair (a1 x1 rounded, a0 x0 fused); what is left
+ *           column by column, a (x alpha) rounded before it is added.  The last m mod 4 rows: one chain of fused products over all
+ *           columns, times alpha
+ *   dger    t = alpha y_j;  a_ij = t x_i fused into a_ij
+ *   drot    x' = c x fused into the rounded s y;  y' = c y fused into the rounded -(s x)
+ *   dscal   x' = alpha x           dgemm 'T','N' (n x n by n x 1): one chain of fused products in k order
+ * tests/golden/check_gelsd_port.py compares every routine below with the library's own, bit for bit, on random and on recorded
+ * systems; the whole solve is checked against np.linalg.lstsq there and, on any machine, against the committed vectors
+ * tests/golden/lstsq_systems.npz (tests/test_gelsd_port.py).
  */
 #include <float.h>
 #include <math.h>
@@ -53,7 +55,7 @@ static int g_kernel_set = 0;
 void gelsd_set_kernel_set(int s) { g_kernel_set = s; }
 int gelsd_get_kernel_set(void) { return g_kernel_set; }
 
-/* ---- BLAS, as the SkylakeX kernel set computes it --------------------------------------------------------- */
+/* ---- BLAS: the arithmetic that the outputs determine (see above) --------------------------------------------- */
 double gelsd_dnrm2(int n, const double* x, int incx) {
   if (n <= 0) return 0.0;
   long double acc[4] = {0.0L, 0.0L, 0.0L, 0.0L};
@@ -82,17 +84,17 @@ void gelsd_dgemv_t(int m, int n, double alpha, const double* a, int lda, const d
     for (int j = 0; j < n; j++) {
       const double* c = &A_(0, j);
       double t;
-      if (j < n4) { /* dgemv_kernel_4x4: AVX2 FMA, one lane per row residue */
+      if (j < n4) { /* a column of the groups of four: four fused chains */
         double l[4] = {0, 0, 0, 0};
         for (int i = 0; i < m2; i++) l[i & 3] = fma(c[i], x[(size_t)i * incx], l[i & 3]);
         t = (l[0] + l[2]) + (l[1] + l[3]);
-        y[j] = y[j] + t * alpha; /* add_y, unit increment: mulpd, addpd */
-      } else if ((n & 2) && j < n4 + 2) { /* dgemv_kernel_4x2: SSE2, two lanes, no FMA */
+        y[j] = y[j] + t * alpha; /* (rounded before it is added) */
+      } else if ((n & 2) && j < n4 + 2) { /* the pair: two chains of rounded products */
         double l[2] = {0, 0};
         for (int i = 0; i < m2; i++) l[i & 1] = l[i & 1] + c[i] * x[(size_t)i * incx];
         t = l[0] + l[1];
         y[j] = fma(alpha, t, y[j]);
-      } else { /* dgemv_kernel_4x1: SSE2, lanes (r0, r1) | (r2, r3) */
+      } else { /* the last odd column: four chains of rounded products */
         double l[4] = {0, 0, 0, 0};
         for (int i = 0; i < m2; i++) l[i & 3] = l[i & 3] + c[i] * x[(size_t)i * incx];
         t = (l[0] + l[2]) + (l[1] + l[3]);
@@ -122,8 +124,8 @@ void gelsd_dgemv_n(int m, int n, double alpha, const double* a, int lda, const d
   if (m <= 0 || n <= 0 || alpha == 0.0) return;
   const int m2 = m & ~3, n4 = n & ~3;
   if (g_kernel_set == 1) {
-    /* Haswell: the 4x4 microkernel sums two FMA chains, (a0 x0 + a2 x2) + (a1 x1 + a3 x3); the pair kernel (unit stride) a0 x0 + a1 x1;
-     * y = fma(t, alpha, y); single columns as below; the C tails are compiled WITHOUT FMA */
+    /* Haswell: four columns at a time by two fused chains, (a0 x0, a2 x2) + (a1 x1, a3 x3); the pair (unit stride) as two rounded
+     * products; single columns as below; the last rows as one chain of rounded products */
     for (int i = 0; i < m2; i++) {
       double yi = 0.0;
       for (int j = 0; j < n4; j += 4) {
@@ -178,7 +180,7 @@ void gelsd_dger(int m, int n, double alpha, const double* x, int incx, const dou
   if (m <= 0 || n <= 0 || alpha == 0.0) return;
   for (int j = 0; j < n; j++) {
     const double t = alpha * y[(size_t)j * incy];
-    /* Haswell daxpy: blocks of sixteen through the FMA microkernel, the rest multiply and add rounded separately */
+    /* Haswell: fused in the leading blocks of sixteen rows, rounded before the addition in the rest */
     const int mf = g_kernel_set == 1 ? (m & ~15) : m;
     for (int i = 0; i < mf; i++) A_(i, j) = fma(t, x[(size_t)i * incx], A_(i, j));
     for (int i = mf; i < m; i++) A_(i, j) = A_(i, j) + t * x[(size_t)i * incx];
@@ -189,6 +191,24 @@ void gelsd_drot(int n, double* x, int incx, double* y, int incy, double c, doubl
     const double xv = x[(size_t)i * incx], yv = y[(size_t)i * incy];
     x[(size_t)i * incx] = fma(c, xv, s * yv);
     y[(size_t)i * incy] = fma(c, yv, -(s * xv));
+  }
+}
+/* y[0..n) = V^T b, V n x n (dgemm 'T','N' with one column) */
+void gelsd_dgemm_tn(int n, const double* v, const double* b, double* y) {
+  for (int i = 0; i < n; i++) {
+    double acc = 0.0;
+    if (g_kernel_set == 1 && i < (n & ~3)) {
+      /* Haswell: results in groups of four by four fused chains over the leading blocks of eight k (k mod 4), the rest of k into the
+       * first, (q0 + q1) + (q2 + q3); the n mod 4 last results by one chain */
+      double q[4] = {0, 0, 0, 0};
+      const int kb = n & ~7;
+      for (int k = 0; k < kb; k++) q[k & 3] = fma(v[k + (size_t)i * n], b[k], q[k & 3]);
+      for (int k = kb; k < n; k++) q[0] = fma(v[k + (size_t)i * n], b[k], q[0]);
+      acc = (q[0] + q[1]) + (q[2] + q[3]);
+    } else {
+      for (int k = 0; k < n; k++) acc = fma(v[k + (size_t)i * n], b[k], acc);
+    }
+    y[i] = acc;
   }
 }
 
@@ -717,22 +737,7 @@ int gelsd_lstsq(const double* Arow, const double* brow, int M, int N, double* x,
       if (d[i] <= tol) b[i] = 0.0;
       else { dlascl_vec(d[i], 1.0, 1, &b[i], 1); rank++; }
     }
-    /* dgemm('T', 'N', N, 1, N, 1, VT, N, b, ., 0, wk, N) */
-    for (int i = 0; i < N; i++) {
-      double acc = 0.0;
-      if (gelsd_get_kernel_set() == 1 && i < (N & ~3)) {
-        /* Haswell dgemm kernel, rows in groups of four: four accumulators over the leading blocks of eight k (k mod 4), the tail
-         * into the first, (a0 + a1) + (a2 + a3); the n mod 4 last rows one FMA chain */
-        double q[4] = {0, 0, 0, 0};
-        const int kb = N & ~7;
-        for (int k = 0; k < kb; k++) q[k & 3] = fma(vt[k + (size_t)i * N], b[k], q[k & 3]);
-        for (int k = kb; k < N; k++) q[0] = fma(vt[k + (size_t)i * N], b[k], q[0]);
-        acc = (q[0] + q[1]) + (q[2] + q[3]);
-      } else {
-        for (int k = 0; k < N; k++) acc = fma(vt[k + (size_t)i * N], b[k], acc);
-      }
-      wk[i] = acc;
-    }
+    gelsd_dgemm_tn(N, vt, b, wk); /* dgemm('T', 'N', N, 1, N, 1, VT, N, b, ., 0, wk, N) */
     for (int i = 0; i < N; i++) b[i] = wk[i];
     dlascl_vec(1.0, orgnrm, N, d, 1);
     /* dlasrt('D'): d is used only for the singular values handed back */

@@ -8,8 +8,8 @@
  * file follows its operation order.  Known sources of last-bit ambiguity that no restatement
  * can pin down: np.dot / np.linalg.norm go through the BLAS ddot of whatever OpenBLAS kernel
  * the host selects (FMA or not), and np.linalg.lstsq is LAPACK gelsd (>= 3 supporters without
- * a "direct" one; 0.13 % of visits).  Here dot products take the FMA form of
- * OpenBLAS' ddot as built for AVX-512 hosts (dot2 below; its build for AVX2 hosts does NOT fuse: lstsq mode 2) and the
+ * a "direct" one; 0.13 % of visits).  Here dot products take the fused form
+ * that np.dot shows on AVX-512 hosts (dot2 below; on AVX2 hosts it does NOT fuse: lstsq mode 2) and the
  * least-squares problem is solved by a one-sided Jacobi SVD (minimum-norm) or, in lstsq modes 1 / 2, as LAPACK dgelsd solves it
  * (pct_oracle_gelsd.c).  Parity status: pinned on the setting-1 fixtures of
  * tests/golden/gen_golden.py (observations, rewards, dones identical over the recorded
@@ -39,16 +39,14 @@
 
 #include "pct_oracle_internal.h"
 
-/* np.dot of two 2-vectors as NumPy's BLAS computes it: OpenBLAS' ddot kernel for AVX-512 hosts ("SkylakeX": the build this
- * oracle was pinned against dispatches to it) accumulates
- * acc = x0*y0; acc = fma(x1, y1, acc) -- ONE rounding for the second product and the sum, not two.  Measured
- * against np.dot on 200 000 random pairs (0 disagreements; the two-rounding form disagrees on 40 %).  It
- * decides the exactly-degenerate tests downstream (a stack centre on the line through a polygon edge). */
-/* (...on hosts where OpenBLAS runs its SkylakeX kernel set -- AVX-512, the build container.  Its "Haswell" kernel set -- AVX2 hosts, AMD
- * Zen included -- compiles that ddot's tail loop WITHOUT FMA: x0*y0 + x1*y1, three roundings; measured under OPENBLAS_CORETYPE=HASWELL,
- * 20 000 of 20 000.  stab_set_lstsq_mode(2) selects that flavour together with the Haswell BLAS arithmetic of pct_oracle_gelsd.c.) */
+/* np.dot of two 2-vectors as NumPy's BLAS returns it: on AVX-512 hosts ("SkylakeX" kernel set) the second product is fused into
+ * the first one -- ONE rounding for the second product and the sum, not two -- and on AVX2 hosts ("Haswell") both are rounded:
+ * np.dot with factors that tell the two apart, tests/golden/derive_blas_orders.py.  It decides the exactly-degenerate tests
+ * downstream (a stack centre on the line through a polygon edge).  stab_set_lstsq_mode(2) selects the second flavour together with
+ * that kernel set's arithmetic in pct_oracle_gelsd.c. */
 static int g_dot_plain = 0;
 static double dot2(double x0, double x1, double y0, double y1) { return g_dot_plain ? x0 * y0 + x1 * y1 : fma(x1, y1, x0 * y0); }
+double stab_dot2_host(double x0, double x1, double y0, double y1) { return dot2(x0, x1, y0, y1); } /* (for the derivation above) */
 
 typedef struct { double c[3]; double m; } sstack;
 typedef struct { int box; double area[4]; double c2[2]; } sdown; /* DownEdge */

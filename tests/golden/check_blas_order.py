@@ -10,8 +10,8 @@ Two probes per pair (i, j) of the terms of one sum, everything else chosen so th
             where the product was rounded before it was added, else its rounding error (with a sign that says which of the two).
 
 Both are taken of the library's routine and of the restatement for every shape up to the sizes below and compared entry by entry.
-dnrm2 adds squares, which cannot cancel: there the order is probed with one large term and the rest so small that what survives
-depends on which partial sum a term goes to.
+dnrm2 adds squares, which cannot cancel; the probes of it here compare results only, and other orders return the same ones.  What
+determines its order, dgemm's and np.dot's is derive_blas_orders.py.
 
     PYTHONDONTWRITEBYTECODE=1 python tests/golden/check_blas_order.py
 """
