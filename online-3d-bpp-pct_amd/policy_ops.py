@@ -132,23 +132,31 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _whole(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _rows_of(x):
     """x with unit stride along the last dimension (itself where it has it)"""
     return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
 
 
-def _mask_args(name, mask, shape):
-    """(tensor, row stride, column stride, type) of a mask that broadcasts to `shape`"""
+def _mask_of(name, mask, shape):
+    """a mask that broadcasts to `shape`, expanded to it (or None)"""
     if mask is None:
-        return None, 0, 0, 0
-    kind = _MASK.get(mask.dtype)
-    if kind is None:
+        return None
+    if mask.dtype not in _MASK:
         raise TypeError("%s: the mask must be bool, uint8, int8, int32 or a 16 / 32-bit float, not %s" % (name, mask.dtype))
     if mask.shape != shape:
         if mask.dim() > 2 or any(a != 1 and a != b for a, b in zip(reversed(mask.shape), reversed(shape))):
             raise ValueError("%s: a mask of shape %s does not fit %s" % (name, tuple(mask.shape), tuple(shape)))
         mask = mask.expand(shape)
-    return mask, mask.stride(0), mask.stride(1), kind
+    return mask
+
+
+def _mask_fields(mask):
+    """address, strides and type of the tensor at hand: a saved mask may come back laid out in another way"""
+    return (None, 0, 0, 0) if mask is None else (mask.data_ptr(), mask.stride(0), mask.stride(1), _MASK[mask.dtype])
 
 
 def _check_logits(name, logits):
@@ -183,7 +191,7 @@ def pick_actions(logits, mask=None, noise=None, actions_out=None, log_probs_out=
     _check_logits("pick_actions", logits)
     n, v = logits.shape
     x = _rows_of(logits)
-    mask, m_row, m_col, m_type = _mask_args("pick_actions", mask, logits.shape)
+    mask = _mask_of("pick_actions", mask, logits.shape)
     if noise is not None:
         if noise.dtype != torch.float32 or noise.shape != logits.shape:
             raise ValueError("pick_actions: noise must be float32 of the logits' shape")
@@ -196,7 +204,7 @@ def pick_actions(logits, mask=None, noise=None, actions_out=None, log_probs_out=
         L = _library()
         ws_bytes = L.pct_choice_workspace(n, v, 0)
         ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
-        c = _Choice(_CHOICE_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask), m_row, m_col, m_type, 0, None,
+        c = _Choice(_CHOICE_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), *_mask_fields(mask), 0, None,
                     0, 0, _ptr(noise), noise.stride(0) if noise is not None else 0, actions.data_ptr(), log_probs.data_ptr(),
                     entropy.data_ptr(), None, None, None, _ptr(ws), ws_bytes)
         _call(L.pct_choice_pick, c, dev)
@@ -216,7 +224,7 @@ def _log_probs_forward(x, given, mask, top, want_stats):
         L = _library()
         ws_bytes = L.pct_choice_workspace(n, v, top)
         ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
-        c = _Choice(_CHOICE_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask[0]), mask[1], mask[2], mask[3],
+        c = _Choice(_CHOICE_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), *_mask_fields(mask),
                     g, given.data_ptr(), top, 0, None, 0, None, log_probs.data_ptr(), entropy.data_ptr(), _ptr(top_log_probs),
                     _ptr(top_actions), _ptr(stats), _ptr(ws), ws_bytes)
         _call(L.pct_choice_log_probs, c, dev)
@@ -225,11 +233,10 @@ def _log_probs_forward(x, given, mask, top, want_stats):
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, given, mask, m_row, m_col, m_type, top):
+    def forward(ctx, logits, given, mask, top):
         x = _rows_of(logits)
-        log_probs, entropy, top_log_probs, top_actions, stats = _log_probs_forward(x, given, (mask, m_row, m_col, m_type), top, True)
+        log_probs, entropy, top_log_probs, top_actions, stats = _log_probs_forward(x, given, mask, top, True)
         ctx.save_for_backward(x, given, mask, top_actions, stats)
-        ctx.mask_args = (m_row, m_col, m_type)
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(top_actions)
@@ -239,17 +246,17 @@ class _LogProbs(torch.autograd.Function):
     @staticmethod
     @_once_differentiable
     def backward(ctx, d_log_probs, d_entropy, d_top=None, _=None):
-        x, given, mask, top_actions, stats = ctx.saved_tensors
+        x, given, mask, top_actions, stats = ctx.saved_tensors  # (hooks on saved tensors may have laid them out anew)
+        x, given, top_actions, stats = _rows_of(x), _whole(given), _whole(top_actions), _whole(stats)
         n, v = x.shape
         dx = x.new_empty((n, v))
         if n:
-            d_log_probs, d_entropy, d_top = (None if t is None else t.contiguous() for t in (d_log_probs, d_entropy, d_top))
-            m_row, m_col, m_type = ctx.mask_args
-            c = _ChoiceGrad(_GRAD_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), _ptr(mask), m_row, m_col, m_type,
+            d_log_probs, d_entropy, d_top = _whole(d_log_probs), _whole(d_entropy), _whole(d_top)
+            c = _ChoiceGrad(_GRAD_SIZE, _DTYPE[x.dtype], n, v, x.data_ptr(), x.stride(0), *_mask_fields(mask),
                             given.shape[1], given.data_ptr(), 0 if top_actions is None else top_actions.shape[1], 0, _ptr(top_actions),
                             stats.data_ptr(), _ptr(d_log_probs), _ptr(d_entropy), _ptr(d_top), dx.data_ptr())
             _call(_library().pct_choice_backward, c, x.device)
-        return dx, None, None, None, None, None, None
+        return dx, None, None, None
 
 
 def action_log_probs(logits, actions, mask=None, top=0):
@@ -275,14 +282,14 @@ def action_log_probs(logits, actions, mask=None, top=0):
     top = int(top)
     if not 0 <= top <= MAX_TOP:
         raise ValueError("action_log_probs: top must be 0 .. %d" % MAX_TOP)
-    mask, m_row, m_col, m_type = _mask_args("action_log_probs", mask, logits.shape)
+    mask = _mask_of("action_log_probs", mask, logits.shape)
     _on_gpu("action_log_probs", logits, actions, mask)
     if given.dtype != torch.int64 or not given.is_contiguous():
         given = given.to(torch.int64).contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        res = _LogProbs.apply(logits, given, mask, m_row, m_col, m_type, top)
+        res = _LogProbs.apply(logits, given, mask, top)
     else:
-        res = _log_probs_forward(_rows_of(logits), given, (mask, m_row, m_col, m_type), top, False)
+        res = _log_probs_forward(_rows_of(logits), given, mask, top, False)
     return ActionLogProbs(res[0] if actions.dim() == 2 else res[0].squeeze(1), res[1], res[2] if top else None, res[3] if top else None)
 
 
@@ -308,10 +315,10 @@ def _strides(x):
 
 
 def _attention_struct(q, k, v, mask, lengths, scale, out, stats, key_list):
-    """mask: (tensor, row stride, column stride, type); the backward reads key_list alone, and says so with any address and type"""
+    """mask: address, row stride, column stride, type; the backward reads key_list alone, and says so with any address and type"""
     b, lq, h, d = q.shape
     return _Attention(_ATTENTION_SIZE, _DTYPE[q.dtype], b, lq, k.shape[1], h, k.shape[2], d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                      _strides(q), _strides(k), _strides(v), _ptr(mask[0]), mask[1], mask[2], mask[3],
+                      _strides(q), _strides(k), _strides(v), *mask,
                       0 if lengths is None else lengths.element_size(), _ptr(lengths), scale, 0, out.data_ptr(), _ptr(stats), _ptr(key_list))
 
 
@@ -329,10 +336,10 @@ def _attend_forward(q, k, v, mask, lengths, scale, want_stats):
     dev, hk = q.device, k.shape[2]
     out = q.new_empty((b, lq, h, d))
     stats = q.new_empty(b * lq * h * 2, dtype=torch.float32) if want_stats else None
-    key_list = q.new_empty((b, k.shape[1] + 1), dtype=torch.int32) if mask[0] is not None else None
+    key_list = q.new_empty((b, k.shape[1] + 1), dtype=torch.int32) if mask is not None else None
     if b and lq:
         L = _library()
-        a = _attention_struct(q, k, v, mask, lengths, scale, out, stats, key_list)
+        a = _attention_struct(q, k, v, _mask_fields(mask), lengths, scale, out, stats, key_list)
         ws = _workspace(L, a, 0, q)  # noqa: F841  (held until the call has been enqueued)
         _call(L.pct_attend, a, dev)
     return out, stats, key_list
@@ -340,9 +347,9 @@ def _attend_forward(q, k, v, mask, lengths, scale, want_stats):
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, mask, m_row, m_col, m_type, lengths, scale):
+    def forward(ctx, q, k, v, mask, lengths, scale):
         q, k, v = _attention_rows(q), _attention_rows(k), _attention_rows(v)
-        out, stats, key_list = _attend_forward(q, k, v, (mask, m_row, m_col, m_type), lengths, scale, True)
+        out, stats, key_list = _attend_forward(q, k, v, mask, lengths, scale, True)
         # (the backward reads the list the forward made of the mask, never the mask itself)
         ctx.save_for_backward(q, k, v, lengths, out, stats, key_list)
         ctx.scale = scale
@@ -352,17 +359,18 @@ class _CrossAttention(torch.autograd.Function):
     @_once_differentiable
     def backward(ctx, d_out):
         q, k, v, lengths, out, stats, key_list = ctx.saved_tensors
-        d_out = _attention_rows(d_out)
+        q, k, v, d_out = _attention_rows(q), _attention_rows(k), _attention_rows(v), _attention_rows(d_out)
+        lengths, out, stats, key_list = _whole(lengths), _whole(out), _whole(stats), _whole(key_list)
         dev = q.device
         d_q, d_k, d_v = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         if q.shape[0]:
             L = _library()
-            a = _attention_struct(q, k, v, (key_list, 0, 0, 4), lengths, ctx.scale, out, stats, key_list)
+            a = _attention_struct(q, k, v, (_ptr(key_list), 0, 0, 4), lengths, ctx.scale, out, stats, key_list)
             a.d_out, a.d_out_stride = d_out.data_ptr(), _strides(d_out)
             a.d_q, a.d_k, a.d_v = d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr()
             ws = _workspace(L, a, 1, q)  # noqa: F841
             _call(L.pct_attend_backward, a, dev)
-        return d_q, d_k, d_v, None, None, None, None, None, None
+        return d_q, d_k, d_v, None, None, None
 
 
 def cross_attention(q, k, v, key_mask=None, key_lengths=None, scale=None):
@@ -395,8 +403,8 @@ def cross_attention(q, k, v, key_mask=None, key_lengths=None, scale=None):
         if key_lengths.dtype not in (torch.int32, torch.int64) or key_lengths.shape != (b,):
             raise ValueError("%s: key_lengths must be int32 or int64 [B]" % name)
         key_lengths = key_lengths.contiguous()
-    mask, m_row, m_col, m_type = _mask_args(name, key_mask, torch.Size((b, lk)))
+    mask = _mask_of(name, key_mask, torch.Size((b, lk)))
     _on_gpu(name, q, k, v, key_mask, key_lengths)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _CrossAttention.apply(q, k, v, mask, m_row, m_col, m_type, key_lengths, scale)
-    return _attend_forward(_attention_rows(q), _attention_rows(k), _attention_rows(v), (mask, m_row, m_col, m_type), key_lengths, scale, False)[0]
+        return _CrossAttention.apply(q, k, v, mask, key_lengths, scale)
+    return _attend_forward(_attention_rows(q), _attention_rows(k), _attention_rows(v), mask, key_lengths, scale, False)[0]

@@ -1,0 +1,77 @@
+"""CPU: what the policy operators hand to the C entries, forward and backward (the calls are caught, nothing is launched)."""
+import importlib
+
+import pytest
+import torch
+
+
+def _ops():
+    return importlib.import_module("online-3d-bpp-pct_amd.policy_ops")
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """the structs of the C calls, in order; tensors may be on the CPU"""
+    seen = []
+    monkeypatch.setattr(_ops(), "_on_gpu", lambda name, *tensors: tensors[0].device)
+    monkeypatch.setattr(_ops(), "_call", lambda fn, args, device: seen.append(args))
+    return seen
+
+
+def _elements(address, tensors):
+    """how many elements lie from `address` to the end of the tensor's storage that holds it"""
+    for t in tensors:
+        s = t.untyped_storage()
+        if s.data_ptr() <= address < s.data_ptr() + s.nbytes():
+            return (s.data_ptr() + s.nbytes() - address) // t.element_size()
+    raise AssertionError("an address of no tensor")
+
+
+@pytest.mark.parametrize("shape", ["column", "row", "shared", "whole"])
+def test_a_saved_mask_may_come_back_in_another_layout(calls, shape):
+    """hooks on saved tensors (offloading, compression) return copies: the backward goes by the copy's strides, not the forward's"""
+    n, v = 64, 50
+    wide = torch.ones(n, 131, 9)
+    mask = {"column": wide[:, 80:130, 8], "row": torch.ones(n, 1), "shared": torch.ones(1, v), "whole": torch.ones(n, v)}[shape]
+    x = torch.zeros(n, v, requires_grad=True)
+    kept = []
+
+    def unpack(t):
+        kept.append(t.clone(memory_format=torch.contiguous_format))
+        return kept[-1]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        out = _ops().action_log_probs(x, torch.zeros(n, dtype=torch.int64), mask=mask)
+    out.log_probs.sum().backward()
+    f, b = calls
+    assert (f.mask_row, f.mask_col) == mask.expand(n, v).stride()
+    held = [t for t in kept if t.data_ptr() == b.mask]
+    assert len(held) == 1 and (b.mask_row, b.mask_col) == held[0].stride()
+    assert (n - 1) * b.mask_row + (v - 1) * b.mask_col < _elements(b.mask, kept)
+
+
+def test_saved_tensors_of_any_layout(calls):
+    """what the kernels take for contiguous is made so, whatever a hook returns"""
+    def other(t):  # the same values, the last dimension far apart
+        if t.dim() < 2:
+            return t.repeat_interleave(2)[::2]
+        return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+    kept = []
+
+    def unpack(t):
+        kept.append(other(t))
+        return kept[-1]
+    x = torch.randn(6, 5, requires_grad=True)
+    q, k, v = (torch.randn(2, l, 3, 16, requires_grad=True) for l in (4, 7, 7))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        a = _ops().action_log_probs(x, torch.zeros(6, 2, dtype=torch.int64), mask=torch.ones(6, 5), top=3)
+        o = _ops().cross_attention(q, k, v, key_mask=torch.ones(2, 7))
+    (a.log_probs.sum() + a.top_log_probs.sum()).backward()
+    c = calls[-1]
+    assert c.logits_row == 5 and (c.mask_row, c.mask_col) == (1, 6)
+    apart = [t.data_ptr() for t in kept if not t.is_contiguous() and t.shape != (6, 5)]
+    assert not {c.logits, c.given, c.stats, c.top_actions} & set(apart)
+    del kept[:]
+    o.sum().backward()
+    c = calls[-1]
+    assert not {c.q, c.k, c.v, c.out, c.stats, c.key_list} & {t.data_ptr() for t in kept if not t.is_contiguous()}
+    assert list(c.q_stride) == [4 * 3 * 16, 3 * 16, 16] and list(c.k_stride) == [7 * 3 * 16, 3 * 16, 16]
