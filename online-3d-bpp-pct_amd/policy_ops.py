@@ -269,7 +269,7 @@ def action_log_probs(logits, actions, mask=None, top=0):
     gradient; an id outside of [-1, V) has NaN.  A row that allows nothing has log-probabilities and entropy 0 and a zero
     gradient.  Alternatives come in falling order, the lower index first among equal logits; where fewer than K choices are
     allowed the rest is -inf with action -1.  The backward pass reads the logits and the mask again: neither may have been
-    written over by then."""
+    written over by then.  The actions may: where a gradient can be asked for, a copy of them is kept."""
     _check_logits("action_log_probs", logits)
     n = logits.shape[0]
     if actions.dtype not in _INTS:
@@ -284,9 +284,12 @@ def action_log_probs(logits, actions, mask=None, top=0):
         raise ValueError("action_log_probs: top must be 0 .. %d" % MAX_TOP)
     mask = _mask_of("action_log_probs", mask, logits.shape)
     _on_gpu("action_log_probs", logits, actions, mask)
+    taped = torch.is_grad_enabled() and logits.requires_grad
     if given.dtype != torch.int64 or not given.is_contiguous():
         given = given.to(torch.int64).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    elif taped:  # (the caller's own, a rollout's slots for instance, which kernels write without telling torch)
+        given = given.clone()
+    if taped:
         res = _LogProbs.apply(logits, given, mask, top)
     else:
         res = _log_probs_forward(_rows_of(logits), given, mask, top, False)
@@ -350,8 +353,8 @@ class _CrossAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, mask, lengths, scale):
         q, k, v = _attention_rows(q), _attention_rows(k), _attention_rows(v)
         out, stats, key_list = _attend_forward(q, k, v, mask, lengths, scale, True)
-        # (the backward reads the list the forward made of the mask, never the mask itself)
-        ctx.save_for_backward(q, k, v, lengths, out, stats, key_list)
+        # (the backward reads the list the forward made of the mask and the lengths, or the lengths alone, never the mask)
+        ctx.save_for_backward(q, k, v, None if key_list is not None else lengths, out, stats, key_list)
         ctx.scale = scale
         return out
 
@@ -382,7 +385,8 @@ def cross_attention(q, k, v, key_mask=None, key_lengths=None, scale=None):
     j < `key_lengths`[b] (int32 or int64 [B]; values outside of [0, Lk] count as the nearer end).  What stands in keys and
     values that are not allowed does not matter, NaN included.  A batch that allows no key gives zeros and takes no gradient.
     Lk, and Lq * H / Hk, are below 2^29, and a call is refused whose launch would hold more than 2^32 threads (some 2^26
-    heads times groups of 32 rows).  The mask may be written over once the call has returned to its stream's order.
+    heads times groups of 32 rows).  The mask and the lengths may be written over once the call has returned, in its stream's
+    order: the backward pass reads what was made of them.
     `scale` is positive, 1 / sqrt(D) if not given.  q, k, v and the output's gradient are read where they are if their rows
     are contiguous and start on 16 bytes, else from a copy."""
     name = "cross_attention"
@@ -406,5 +410,7 @@ def cross_attention(q, k, v, key_mask=None, key_lengths=None, scale=None):
     mask = _mask_of(name, key_mask, torch.Size((b, lk)))
     _on_gpu(name, q, k, v, key_mask, key_lengths)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        if key_lengths is not None and mask is None:
+            key_lengths = key_lengths.clone()  # (the backward reads them again)
         return _CrossAttention.apply(q, k, v, mask, key_lengths, scale)
     return _attend_forward(_attention_rows(q), _attention_rows(k), _attention_rows(v), mask, key_lengths, scale, False)[0]

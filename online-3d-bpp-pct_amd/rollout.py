@@ -86,12 +86,15 @@ class RolloutSlots(object):
     def evaluate(self, logits, top=0):
         """What an update needs of the stored steps: `action_log_probs` of the stored actions under `logits` [T * N, L] (or
         [T, N, L]), computed by the caller's policy from `obs[:-1]`, over each observation's valid leaves.  Log-probabilities
-        come as [T * N, 1], the entropy as [T * N]; differentiable with respect to `logits`."""
+        come as [T * N, 1], the entropy as [T * N]; differentiable with respect to `logits`.  What the backward pass reads of the
+        slots is copied; what the caller's policy keeps of `obs` for its own is not, so take it before the next `collect`."""
         rows = self.num_steps * self.actions.shape[1]
         logits = logits.reshape(-1, logits.shape[-1])
         if logits.shape[0] != rows:
             raise ValueError("evaluate: logits of %d rows for %d stored actions" % (logits.shape[0], rows))
         mask = leaf_mask(self.obs[:-1].view(rows, -1, 9), logits.shape[1])
+        if torch.is_grad_enabled() and logits.requires_grad:
+            mask = mask != 0  # a copy (of one byte to an entry): the kernels of later steps write the slots without telling torch
         return action_log_probs(logits, self.actions.view(rows, 1), mask=mask, top=top)
 
     def gather(self, group=None):

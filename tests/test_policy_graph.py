@@ -1,4 +1,5 @@
 """CPU: what the policy operators hand to the C entries, forward and backward (the calls are caught, nothing is launched)."""
+import ctypes
 import importlib
 
 import pytest
@@ -75,3 +76,42 @@ def test_saved_tensors_of_any_layout(calls):
     c = calls[-1]
     assert not {c.q, c.k, c.v, c.out, c.stats, c.key_list} & {t.data_ptr() for t in kept if not t.is_contiguous()}
     assert list(c.q_stride) == [4 * 3 * 16, 3 * 16, 16] and list(c.k_stride) == [7 * 3 * 16, 3 * 16, 16]
+
+
+def test_the_backward_reads_its_own_copy_of_actions_and_lengths(calls):
+    """kernels write a rollout's slots through their addresses, which torch's version counters do not see"""
+    slots = torch.randint(0, 5, (3, 4, 1))
+    x = torch.randn(12, 5, requires_grad=True)
+    out = _ops().action_log_probs(x, slots.view(12, 1))
+    was = slots.clone()
+    slots.untyped_storage().fill_(1)  # (as a kernel does: no version is counted)
+    out.log_probs.sum().backward(retain_graph=True)  # (the copy lives as long as the graph)
+    assert not slots.data_ptr() <= calls[-1].given < slots.data_ptr() + slots.nbytes
+    assert ctypes.string_at(calls[-1].given, slots.nbytes) == was.numpy().tobytes()
+    q, k, v = (torch.randn(2, l, 1, 8, requires_grad=True) for l in (3, 6, 6))
+    lengths = torch.tensor([4, 6])
+    out = _ops().cross_attention(q, k, v, key_lengths=lengths)
+    lengths.untyped_storage().fill_(0)
+    out.sum().backward(retain_graph=True)
+    assert ctypes.string_at(calls[-1].key_lengths, 16) == torch.tensor([4, 6]).numpy().tobytes()
+    out = _ops().cross_attention(q, k, v, key_mask=torch.ones(2, 6), key_lengths=lengths)
+    lengths.fill_(1)  # (written over in torch's sight: the list of keys was made already)
+    out.sum().backward()
+    assert calls[-1].key_lengths is None and calls[-1].key_list
+
+
+def test_an_evaluation_reads_its_own_copy_of_the_slots(calls):
+    r = importlib.import_module("online-3d-bpp-pct_amd").RolloutSlots(3, 2, (14 * 9,), 1.0, "cpu")
+    r.obs.view(4, 2, 14, 9)[:, :, 9:12, 8] = 1.0
+    logits = torch.randn(6, 5, requires_grad=True)
+    res = r.evaluate(logits)
+    r.obs.untyped_storage().fill_(1)
+    r.actions.untyped_storage().fill_(1)
+    res.log_probs.sum().backward(retain_graph=True)
+    f, b = calls
+    assert f.mask == b.mask and (b.mask_row, b.mask_col, b.mask_type) == (5, 1, 1)
+    assert ctypes.string_at(b.mask, 30) == bytes([0, 1, 1, 1, 0]) * 6
+    assert ctypes.string_at(b.given, 48) == bytes(48)
+    with torch.no_grad():  # without a gradient the observation's own column is read where it is
+        r.evaluate(logits)
+    assert calls[-1].mask == r.obs.view(-1, 14, 9)[0, 8:, 8].data_ptr()
