@@ -208,6 +208,9 @@ def pick_actions(logits, mask=None, noise=None, actions_out=None, log_probs_out=
                     0, 0, _ptr(noise), noise.stride(0) if noise is not None else 0, actions.data_ptr(), log_probs.data_ptr(),
                     entropy.data_ptr(), None, None, None, _ptr(ws), ws_bytes)
         _call(L.pct_choice_pick, c, dev)
+        for t in (actions_out, log_probs_out):
+            if t is not None:  # written in place: a graph that has saved it says so instead of reading the new values
+                torch.autograd.graph.increment_version(t)
     return PickedActions(actions, log_probs, entropy)
 
 

@@ -115,3 +115,18 @@ def test_an_evaluation_reads_its_own_copy_of_the_slots(calls):
     with torch.no_grad():  # without a gradient the observation's own column is read where it is
         r.evaluate(logits)
     assert calls[-1].mask == r.obs.view(-1, 14, 9)[0, 8:, 8].data_ptr()
+
+
+def test_outputs_written_in_place_are_counted(calls):
+    """a graph of torch's own that has saved the slot refuses its backward pass, as after any in-place operation"""
+    slots = torch.zeros(4, 6, 1, dtype=torch.int64)
+    lps = torch.zeros(4, 6, 1)
+    x = torch.randn(6, 5, requires_grad=True)
+    own = torch.log_softmax(x, 1).gather(1, slots[2])
+    _ops().pick_actions(x.detach(), actions_out=slots[2], log_probs_out=lps[2])
+    assert slots._version == 1 and lps._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        own.sum().backward()
+    _ops().pick_actions(torch.zeros(0, 5), actions_out=slots[:, :0, 0].reshape(-1))
+    with torch.inference_mode():  # (these have no counter)
+        _ops().pick_actions(torch.zeros(6, 5), actions_out=torch.zeros(6, dtype=torch.int64))
