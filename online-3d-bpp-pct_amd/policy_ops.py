@@ -21,6 +21,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .vec_env import PctEnvError
@@ -126,6 +127,13 @@ def _on_gpu(name, *tensors):
                 raise PctEnvError("%s runs on an AMD GPU only (a tensor is on %s); there is no CPU path" % (name, t.device))
             raise ValueError("%s: tensors on %s and on %s" % (name, dev, t.device))
     return dev
+
+
+def _no_tangents(name, *tensors):
+    """the kernels differentiate backward only: a forward-mode derivative would be lost on the way"""
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("%s: forward-mode derivatives are not implemented" % name)
 
 
 def _ptr(t):
@@ -266,7 +274,7 @@ def action_log_probs(logits, actions, mask=None, top=0):
     """Log-probabilities of given choices under softmax(logits) over the allowed choices (`pick_actions` says which), the
     entropy of each row and, with `top` = K (at most 64), its K best choices.  Returns `ActionLogProbs(log_probs, entropy [N],
     top_log_probs [N, K] or None, top_actions int64 [N, K] or None)`, the log-probabilities float32 and in the shape of
-    `actions`, integers [N] or [N, G], G at most 64.  Differentiable with respect to `logits` (once).
+    `actions`, integers [N] or [N, G], G at most 64.  Differentiable with respect to `logits` (once, backward).
 
     An id of -1 stands for "none": log-probability 0, no gradient.  A choice that is not allowed has -inf and takes no
     gradient; an id outside of [-1, V) has NaN.  A row that allows nothing has log-probabilities and entropy 0 and a zero
@@ -287,6 +295,7 @@ def action_log_probs(logits, actions, mask=None, top=0):
         raise ValueError("action_log_probs: top must be 0 .. %d" % MAX_TOP)
     mask = _mask_of("action_log_probs", mask, logits.shape)
     _on_gpu("action_log_probs", logits, actions, mask)
+    _no_tangents("action_log_probs", logits)
     taped = torch.is_grad_enabled() and logits.requires_grad
     if given.dtype != torch.int64 or not given.is_contiguous():
         given = given.to(torch.int64).contiguous()
@@ -382,7 +391,7 @@ class _CrossAttention(torch.autograd.Function):
 def cross_attention(q, k, v, key_mask=None, key_lengths=None, scale=None):
     """softmax(scale q k^T) v over the allowed keys of each batch: q [B, Lq, H, D], k and v [B, Lk, Hk, D], one of float32,
     bfloat16 and float16; H a multiple of Hk (H / Hk heads in a row share a key/value head), D a multiple of 8 up to 128; any
-    lengths.  Returns [B, Lq, H, D] (contiguous), differentiable with respect to q, k and v (once).
+    lengths.  Returns [B, Lq, H, D] (contiguous), differentiable with respect to q, k and v (once, backward).
 
     Key j of batch b is allowed where `key_mask` [B, Lk] (any strides: the observation's mask column will do) is not zero and
     j < `key_lengths`[b] (int32 or int64 [B]; values outside of [0, Lk] count as the nearer end).  What stands in keys and
@@ -412,6 +421,7 @@ def cross_attention(q, k, v, key_mask=None, key_lengths=None, scale=None):
         key_lengths = key_lengths.contiguous()
     mask = _mask_of(name, key_mask, torch.Size((b, lk)))
     _on_gpu(name, q, k, v, key_mask, key_lengths)
+    _no_tangents(name, q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if key_lengths is not None and mask is None:
             key_lengths = key_lengths.clone()  # (the backward reads them again)

@@ -130,3 +130,21 @@ def test_outputs_written_in_place_are_counted(calls):
     _ops().pick_actions(torch.zeros(0, 5), actions_out=slots[:, :0, 0].reshape(-1))
     with torch.inference_mode():  # (these have no counter)
         _ops().pick_actions(torch.zeros(6, 5), actions_out=torch.zeros(6, dtype=torch.int64))
+
+
+def test_forward_mode_derivatives_are_refused(calls):
+    """with and without a graph: outputs without a tangent would pass for constants"""
+    from torch.autograd import forward_ad
+    ids = torch.zeros(3, dtype=torch.int64)
+    for graph in (False, True):
+        with forward_ad.dual_level():
+            dual = lambda *s: forward_ad.make_dual(torch.randn(*s, requires_grad=graph), torch.ones(*s))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                _ops().action_log_probs(dual(3, 5), ids)
+            for at in range(3):
+                args = [dual(2, l, 1, 8) if i == at else torch.randn(2, l, 1, 8) for i, l in enumerate((3, 4, 4))]
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    _ops().cross_attention(*args)
+            assert not calls
+            _ops().action_log_probs(torch.zeros(3, 5), ids)  # others may pass within the level
+            del calls[:]
