@@ -14,4 +14,4 @@ from .lstsq_mode import numpy_lstsq_mode, numpy_blas  # noqa: F401
 
 __all__ = ["PctVecEnv", "PctEnvError", "VecEnv", "LazyInfos", "make_vec_envs", "shard_envs", "gather_rollout",
            "DeviceRollout", "RolloutSlots", "collect", "get_leaf_nodes", "leaf_mask", "evaluate_heuristic", "HEURISTICS", "numpy_lstsq_mode", "numpy_blas",
-           "pick_actions", "action_log_probs", "cross_attention", "PickedActions", "ActionLogProbs"]
+           "pick_actions", "action_log_probs", "cross_attention", "PickedActions", "ActionLogProbs", "LeafPolicy"]
