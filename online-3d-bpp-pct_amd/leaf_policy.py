@@ -27,13 +27,14 @@ class LeafPolicy(torch.nn.Module):
 
     def forward(self, all_nodes):
         (i, l), n, h = self.holders, all_nodes.shape[0], self.heads
+        d = self.embed.out_features // h
         if all_nodes.dim() != 3 or all_nodes.shape[1:] != (i + l + 1, 9):
             raise ValueError("LeafPolicy: observations must be [N, %d, 9], not %s" % (i + l + 1, tuple(all_nodes.shape)))
         mask = all_nodes[:, :, 8]
         x = self.embed(all_nodes.to(self.embed.weight.dtype)) + self.kinds[self.kind]
-        q, k, v = self.node_qkv(x).view(n, i + l + 1, 3, h, -1).unbind(2)
+        q, k, v = self.node_qkv(x).view(n, i + l + 1, 3, h, d).unbind(2)
         x = x + cross_attention(q, k, v, key_mask=mask).flatten(2)
         leaves = x[:, i:i + l]
-        k, v = self.leaf_kv(x).view(n, i + l + 1, 2, h, -1).unbind(2)
-        seen = cross_attention(self.leaf_q(leaves).view(n, l, h, -1), k, v, key_mask=mask)
+        k, v = self.leaf_kv(x).view(n, i + l + 1, 2, h, d).unbind(2)
+        seen = cross_attention(self.leaf_q(leaves).view(n, l, h, d), k, v, key_mask=mask)
         return self.score(torch.tanh(leaves + seen.flatten(2))).squeeze(2).float()

@@ -17,3 +17,15 @@ def test_every_name_of_the_documents_is_public():
         missing = sorted(n for n in names if not hasattr(pct_amd, n))
         assert names and not missing, (doc, missing)
     assert "LeafPolicy" in pct_amd.__all__
+
+
+def test_an_empty_batch_reaches_the_operators(monkeypatch):
+    """no observations give no logits (heads are split by their width: a size to be inferred is refused for empty tensors)"""
+    ops = importlib.import_module("online-3d-bpp-pct_amd.policy_ops")
+    monkeypatch.setattr(ops, "_on_gpu", lambda name, *tensors: tensors[0].device)
+    monkeypatch.setattr(ops, "_call", lambda *a: pytest.fail("nothing is launched for an empty batch"))
+    net = importlib.import_module("pct_amd").LeafPolicy(8, 5, width=32, heads=2)
+    logits = net(torch.zeros(0, 14, 9))
+    assert logits.shape == (0, 5)
+    logits.sum().backward()
+    assert all(p.grad is not None and not p.grad.any() for p in net.parameters())
