@@ -9,7 +9,8 @@
  *
  * The conventions are those of pct_env.h: int status (PCT_OK == 0, text from pct_last_error()), `stream` is a hipStream_t,
  * work is only enqueued on it, every pointer is device memory on the current device that the caller owns; nothing is
- * allocated, kept or synchronised.  Strides count elements.  Sizes that are zero enqueue nothing.
+ * allocated, kept or synchronised.  Strides count elements.  Sizes that are zero enqueue nothing.  Workspaces and statistics start
+ * on 16 bytes.
  */
 #ifndef PCT_POLICY_H
 #define PCT_POLICY_H

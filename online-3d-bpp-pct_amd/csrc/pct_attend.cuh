@@ -914,10 +914,12 @@ template <typename T> struct Attend {
     if (p.k_len <= 512) mw = p.list || p.lengths ? 2 : 4;
     return cut(p.k_len, (p.rows + Type<T>::ROWS - 1) / Type<T>::ROWS, (int64_t)p.batch * p.kv_heads, mw);
   }
+  // the partial statistics, up to where the partial results start (those are read 16 bytes at a time)
+  static int64_t stats_bytes(int splits, int64_t rows) { return (splits * rows * 8 + 15) / 16 * 16; }
   static int64_t workspace(const AttendParams& p, bool backward) {
     const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows;
     const Cut q = cut_q(p, backward);
-    if (!backward) return q.splits > 1 ? q.splits * rows * (8 + 4 * (int64_t)p.dim) : 0;
+    if (!backward) return q.splits > 1 ? stats_bytes(q.splits, rows) + q.splits * rows * 4 * (int64_t)p.dim : 0;
     const Cut k = cut_k(p);
     const int64_t a = q.splits > 1 ? q.splits * rows * p.dim * 4 : 0;
     const int64_t b = k.splits > 1 ? k.splits * 2 * (int64_t)p.batch * p.k_len * p.kv_heads * p.dim * 4 : 0;
@@ -946,7 +948,7 @@ template <typename T> struct Attend {
     const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows;
     set(p, c, false);
     p.part_stats = (float2*)ws;
-    p.part = (float*)(ws + c.splits * rows * 8);
+    p.part = (float*)(ws + stats_bytes(c.splits, rows));
     dim3 g;
     if (int rc = grid(p, c, false, g)) return rc;
     by_dim(p.dim, [&](auto d) {

@@ -148,3 +148,21 @@ def test_forward_mode_derivatives_are_refused(calls):
             assert not calls
             _ops().action_log_probs(torch.zeros(3, 5), ids)  # others may pass within the level
             del calls[:]
+
+
+def test_partial_results_of_attention_start_on_their_alignment():
+    """the forward's float32 partials follow its statistics in the workspace: both are read 16 bytes at a time"""
+    import ctypes as C
+    ops = _ops()
+    L = ops._library()
+    odd = 0
+    for batch, lq, lk, heads, dim, dtype in ((1, 1, 768, 1, 64, 1), (1, 3, 5000, 1, 8, 0), (1, 1, 16384, 3, 128, 1), (1, 5, 3000, 1, 40, 2), (1, 1, 2048, 1, 16, 0)):
+        a = ops._Attention()
+        a.struct_size = C.sizeof(a)
+        a.batch, a.q_len, a.k_len, a.heads, a.kv_heads, a.dim, a.scale, a.dtype = batch, lq, lk, heads, heads, dim, 1.0, dtype
+        size, rows = L.pct_attend_workspace(C.addressof(a), 0), batch * lq * heads
+        splits = size // (rows * (8 + 4 * dim))  # (the rounding is less than a split's share)
+        assert splits > 1
+        odd += splits * rows % 2
+        assert size - splits * rows * dim * 4 == (splits * rows * 8 + 15) // 16 * 16, (batch, lq, lk, size, splits)
+    assert odd
