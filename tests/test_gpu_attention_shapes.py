@@ -30,6 +30,18 @@ def _check(shape, dtype, kind, seed, train=True):
         _close(g, w, e, (name, shape, kind))
 
 
+# 64 heads and more of at most 512 keys, of which some are not allowed: the key gradient's workgroups are numbered by dies, with
+# places left over where the heads are not a multiple of 8, several tiles of keys, and (the last) several parts of the queries
+BY_DIE = [(67, 9, 131, 1, 1, 32), (33, 5, 300, 2, 2, 64), (13, 3, 512, 5, 5, 16), (71, 40, 97, 2, 1, 128), (66, 300, 300, 2, 1, 16)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("kind", ["lengths", "column", "both"])
+@pytest.mark.parametrize("shape", BY_DIE, ids=str)
+def test_heads_numbered_by_die(shape, kind, dtype):
+    _check(shape, dtype, kind, 40)
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("shape", [(1, 1, 768, 1, 1, 64), (1, 3, 5000, 1, 1, 8), (1, 1, 16384, 3, 3, 128), (1, 5, 3000, 1, 1, 40), (1, 1, 2048, 1, 1, 16)], ids=str)
 def test_an_odd_number_of_partial_rows(shape, dtype):
