@@ -63,6 +63,14 @@ struct AttendParams {
 namespace {
 
 constexpr float kLowest = -3.402823466e38f;
+// What fills up a tile behind the last row: a row's second product meets P = 0 there, which must not make NaN of an infinite value.
+__device__ uint4 kZeroRow[32];  // (128 float32)
+template <typename T>
+__device__ __forceinline__ const T* zero_row() {
+  uint64_t p = (uint64_t)kZeroRow;
+  asm volatile("" : "+s"(p));  // (asked for where it is used: kept in registers over a tile it costs a wavefront of 5 to a SIMD)
+  return (const T*)p;
+}
 
 template <typename T> using Frag = T __attribute__((ext_vector_type(8)));
 typedef float Acc __attribute__((ext_vector_type(16)));
@@ -345,7 +353,7 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
     L::stage2(k, k + KT * DP, p.dim, wave, waves, lane, [&](int r, const T*& a, const T*& b) {
       const int64_t key = keys[t & 1][r];
       a = kb + key * p.ks[1];
-      b = vb + key * p.vs[1];
+      b = t * KT + r >= n ? zero_row<T>() : vb + key * p.vs[1];
     });
   };
   if (p.dim != DP) zero_lds<4 * L::BYTES>(lds, tid, blockDim.x);
@@ -708,11 +716,11 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams 
 
   auto stage = [&](int t) {
     T* q = buf + (t & 1) * 2 * QT * DP;
-    auto at = [&](int r) { r += t * QT; return r < p.rows ? r : p.rows - 1; };
     L::stage2(q, q + QT * DP, p.dim, wave, waves, lane, [&](int r, const T*& a, const T*& b) {
-      const int x = at(r), l = p.group == 1 ? x : (int)p.by_group.of(x), g = x - l * p.group;
+      const bool in = t * QT + r < p.rows;
+      const int x = in ? t * QT + r : p.rows - 1, l = p.group == 1 ? x : (int)p.by_group.of(x), g = x - l * p.group;
       a = qb + l * p.qs[1] + g * p.qs[2];
-      b = db + l * p.ds[1] + g * p.ds[2];
+      b = in ? db + l * p.ds[1] + g * p.ds[2] : zero_row<T>();
     });
   };
   // (a workgroup has at least 64 threads: one to a staged row)

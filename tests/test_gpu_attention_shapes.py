@@ -47,3 +47,31 @@ def test_heads_numbered_by_die(shape, kind, dtype):
 def test_an_odd_number_of_partial_rows(shape, dtype):
     _check(shape, dtype, "none", 41, train=False)
     _check(shape, dtype, "lengths", 42, train=False)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("lq,lk", [(1, 1), (40, 70), (5, 33), (130, 3), (64, 64), (3, 2500), (300, 9)], ids=str)
+def test_infinite_values_and_gradients_stay_in_their_columns(lq, lk, dtype):
+    """an allowed key's infinite value makes its column infinite where it weighs, and so does the output's gradient in dv: at the
+    first, an inner and the last place, behind which a tile is filled up"""
+    d = 40
+    q, k, v, do = _qkv((2, lq, lk, 2, 1, d), dtype, 43)
+    out = _pkg().cross_attention(q, k, v)
+    for at in sorted({0, lk // 2, lk - 1}):
+        w = v.clone()
+        w[1, at, 0, 7] = math.inf
+        w[1, at, 0, 8] = -math.inf
+        got = _pkg().cross_attention(q, k, w)
+        assert (got[1, :, :, 7] == math.inf).all() and (got[1, :, :, 8] == -math.inf).all(), at
+        keep = [i for i in range(d) if i not in (7, 8)]
+        assert torch.equal(got[0], out[0]) and torch.equal(got[1][..., keep], out[1][..., keep]), at
+    leaf = v.clone().requires_grad_(True)
+    want, = torch.autograd.grad(_pkg().cross_attention(q, k, leaf), [leaf], do)
+    for at in sorted({0, lq // 2, lq - 1}):
+        g = do.clone()
+        g[1, at, 1, 7] = -math.inf
+        leaf = v.clone().requires_grad_(True)
+        got, = torch.autograd.grad(_pkg().cross_attention(q, k, leaf), [leaf], g)
+        keep = [i for i in range(d) if i != 7]
+        assert (got[1, :, 0, 7] == -math.inf).all(), at
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1][..., keep], want[1][..., keep]), at
