@@ -340,7 +340,6 @@ struct CGeo {  // placed-box geometry for the stability code
   const double* box;
   const double* bsz;
   int I;
-  static constexpr bool kSquareIsPow = false;  // (pct_stab.cuh, the lever rule's `tri_base_len ** 2`)
   __device__ __forceinline__ void operator()(int i, double g[9]) const {
 #pragma unroll
     for (int c = 0; c < 6; c++) g[c] = box[c * I + i];

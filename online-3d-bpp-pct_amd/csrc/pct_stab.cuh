@@ -49,7 +49,6 @@
 #endif
 
 #include "pct_gelsd.cuh"
-#include "pct_pow.cuh"
 
 namespace pct {
 
@@ -85,6 +84,7 @@ struct StabCaps {
 };
 #if !defined(__HIPCC__)
 static int g_stab_host_gelsd = 1;  // host test build (tests/host): the mode the handle carries in StabCaps on the device
+static int g_stab_host_pow = 0;    // ... and whether lever_square is the C library's pow, as in the reference, instead of what the device runs
 #endif
 
 // per-env stability state: pointers into LDS (device) or host memory
@@ -349,6 +349,21 @@ struct StabDot2 {
   PCT_SM double operator()(double x0, double x1, double y0, double y1) const { return plain ? x0 * y0 + x1 * y1 : fma(x1, y1, x0 * y0); }
 };
 
+// `tri_base_len ** 2` of the lever rule (D/space.py:112,210; C/space.py:108,206).  tri_base_len is an np.float64, whose power is the
+// C library's pow(len, 2.0), and that is not correctly rounded: by calling it, its last bit differs from len * len on about 0.08 % of
+// the continuous env's lengths and on none of a discrete env's up to 43 units per axis (exhaustive; the first is the length of
+// (39.5, 43.5)).  Here the square is the correctly rounded one, so a verdict of the continuous env (or of a bin of more than 43 units
+// per axis) that hangs on that bit may differ from a reference run: tests/test_stab_square.py counts them.
+PCT_SD double lever_square(double len) {
+#if !defined(__HIPCC__)
+  if (g_stab_host_pow) {
+    volatile double two = 2.0;  // (a literal exponent of 2 would be folded into len * len)
+    return pow(len, two);
+  }
+#endif
+  return len * len;
+}
+
 // The same solve with every extent a compile-time constant (N supporters, M = N(N-1)/2 + 1 rows) and every loop over
 // rows, columns and column pairs unrolled: U and V are then registers, not dynamically indexed private arrays in
 // scratch memory.  Operation for operation the generic routine.
@@ -544,10 +559,7 @@ PCT_SD bool stab_split(const Geo& geo, const double bg[9], int k, const Sup& sup
       double t0 = e00 - e10, t1 = e01 - e11;
       const StabDot2 dot2{gelsd_avx2};  // (the lever rule's np.dot / np.linalg.norm follow the host flavour too)
       double len = sqrt(dot2(t0, t1, t0, t1));
-      // tri_base_len ** 2 (pct_pow.cuh).  Geo::kSquareIsPow: every length this env can produce -- sqrt of a sum of two squares
-      // of half-integers below 32 (the 5-bit-coordinate discrete kernels) -- has pow(len, 2.0) == len * len (exhaustive up
-      // to 43 per axis, tests/test_stab_host.py; the first length that differs is that of (39.5, 43.5))
-      double l2 = Geo::kSquareIsPow ? len * len : lever_square(len);
+      const double l2 = lever_square(len);
       t0 /= l2; t1 /= l2;
       sp.f[0] = fabs(dot2(stk[0] - e10, stk[1] - e11, t0, t1));
       sp.f[1] = fabs(dot2(stk[0] - e00, stk[1] - e01, t0, t1));

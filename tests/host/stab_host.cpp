@@ -31,7 +31,6 @@ struct stab {
 
 struct GeoFn {
   const double* g;
-  static constexpr bool kSquareIsPow = false;  // the host flavour always runs the pow restatement
   void operator()(int i, double out[9]) const { memcpy(out, g + 9 * (size_t)i, 9 * sizeof(double)); }
 };
 struct Task { int S; double stk[4]; };
@@ -72,6 +71,9 @@ void stab_set_ill_near(int) {}  // (the tie notice is an analysis mode of the or
 // the product's PCT_LSTSQ_GELSD (csrc/pct_gelsd.cuh compiled for the host) under the oracle's switch
 void stab_set_lstsq_mode(int mode) { pct::g_stab_host_gelsd = mode; }
 int stab_get_lstsq_mode(void) { return pct::g_stab_host_gelsd; }
+// the lever rule's square: what the device runs (0, the default) or the C library's pow (1)
+void stab_host_set_pow(int on) { pct::g_stab_host_pow = on; }
+double stab_host_lever_square(double len) { return pct::lever_square(len); }
 // pct_oracle.h exports the oracle's own restatement under this name; here it is the PRODUCT's solve (geometry-free entry for tests):
 // row-major M x N system with the right-hand side e_M is not what the product takes, so tests/test_stab_host.py uses gelsd_host_split
 int gelsd_lstsq(const double*, const double*, int, int, double*, int*, double*, int*) { return -1; }
@@ -144,9 +146,13 @@ void gelsd_host_dnrm2_certified_sweep(long count, unsigned long long seed, long*
     if (memcmp(&ref, &f, 8)) out[2]++;
   }
 }
-// pct_pow.cuh (glibc's pow as its FMA build executes it) against the live libm, on lengths of the lever rule: `count` values from
-// the continuous env's domain (norms of differences of 1e-6-lattice contact centres halved, i.e. multiples of 5e-7 up to `span`).
-// out[0] = lengths, out[1] = differences to libm's pow(len, 2.0), out[2] = lengths with pow(len, 2.0) != len * len.
+// The lever rule's square (pct_stab.cuh lever_square) and libm's pow, on `count` lengths of the continuous env's domain (norms of
+// differences of 1e-6-lattice contact centres halved, i.e. multiples of 5e-7 up to `span`).  out[0] = lengths, out[1] = lengths whose
+// lever_square is not the correctly rounded square, out[2] = lengths with pow(len, 2.0) != len * len.
+static bool rounded_square(double len, double square) {  // the square's error, exact in one FMA, is at most half an ulp
+  const double err = fma(len, len, -square);
+  return fabs(err) <= 0.5 * (nextafter(square, INFINITY) - square);
+}
 void pow_host_sweep_continuous(long count, unsigned long long seed, double span, long* out) {
   unsigned long long s = seed;
   auto rnd = [&]() { s = s * 6364136223846793005ull + 1442695040888963407ull; return (double)(s >> 11) / 9007199254740992.0; };
@@ -159,14 +165,13 @@ void pow_host_sweep_continuous(long count, unsigned long long seed, double span,
     const double t0 = c0x - c1x, t1 = c0y - c1y;
     const double len = sqrt(fma(t1, t1, t0 * t0));
     if (!(len > 0)) continue;
-    const double a = pow(len, two), b = pct::pow_glibc_fma(len, 2.0);
     out[0]++;
-    if (memcmp(&a, &b, 8)) out[1]++;
-    if (a != len * len) out[2]++;
+    if (!rounded_square(len, pct::lever_square(len))) out[1]++;
+    if (pow(len, two) != len * len) out[2]++;
   }
 }
 // ... and the DISCRETE env's lengths, exhaustively: sqrt(dx^2 + dy^2) for dx, dy multiples of 1/2 up to `side` (contact centres of
-// integer rectangles), both np.dot flavours.  out[0] = lengths, out[1] = pow_glibc_fma != libm, out[2] = libm pow(len, 2.0) != len * len.
+// integer rectangles), both np.dot flavours.  The same three counts.
 void pow_host_sweep_discrete(int side, long* out) {
   out[0] = out[1] = out[2] = 0;
   volatile double two = 2.0;
@@ -176,14 +181,13 @@ void pow_host_sweep_discrete(int side, long* out) {
       const double t0 = i / 2.0, t1 = j / 2.0;
       for (int avx2 = 0; avx2 < 2; avx2++) {
         const double len = sqrt(avx2 ? t0 * t0 + t1 * t1 : fma(t1, t1, t0 * t0));
-        const double a = pow(len, two), b = pct::pow_glibc_fma(len, 2.0);
         out[0]++;
-        if (memcmp(&a, &b, 8)) out[1]++;
-        if (a != len * len) out[2]++;
+        if (!rounded_square(len, pct::lever_square(len))) out[1]++;
+        if (pow(len, two) != len * len) out[2]++;
       }
     }
 }
-double pow_host(double x, double y) { return pct::pow_glibc_fma(x, y); }
+double pow_host(double x, double y) { return pow(x, y); }  // libm's own
 // dbdsqr('U', n, ncvt = n, 0, 1): d[n], e[n - 1], vt[n * n] (column-major), c[n], work[4 n]
 int gelsd_host_dbdsqr(int n, double* d, double* e, double* vt, double* c, double* work) { const pct::gelsd::Grp one = {0, 1}; return pct::gelsd::dbdsqr(one, n, d, e, vt, c, work) ? 0 : 1; }
 
