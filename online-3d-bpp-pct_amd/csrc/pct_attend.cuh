@@ -456,7 +456,9 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
   for (int i = 0; i < DB; i++) store_row<T>(dst + 32 * i, o[i], inv, p.dim - 32 * i, h);
 }
 
-// Joins a few splits of the forward pass: a thread to 4 elements of a row walks over them.
+// Joins the splits of the forward pass: a thread to 4 elements of a row walks over them, four in flight.  Bound by latency: 512 rows of
+// 128 in 16 parts 6.3 us, in 64 parts 13.2, 2048 rows in 32 parts 9.0.  (A wavefront to a row with all of its reads in flight was no
+// faster anywhere: 7.0, 13.0, 9.4, and 10.8 against 8.8 for one row in 64 parts.)
 template <typename T>
 __global__ __launch_bounds__(256) void pct_attend_join_kernel(AttendParams p) {
   const int per = p.dim / 4;
@@ -481,34 +483,6 @@ __global__ __launch_bounds__(256) void pct_attend_join_kernel(AttendParams p) {
   if (d == 0 && p.stats) p.stats[at] = none ? make_float2(0.f, INFINITY) : make_float2(ref, sum);
   const Work w = {bh / p.kv_heads, bh % p.kv_heads, 0, 0};
   store4<T>((T*)p.out + out_head(p, w) + out_row(p, r) + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-}
-
-// Joins many splits, where there are few rows: a wavefront to a row, each half takes every other split, a lane 4 elements, so that
-// all of a row's reads are in flight at once.  Measured, walking / so: 512 rows of 128, 16 splits 15.5 / 7.6 us; 18612 rows of 80,
-// 3 splits 7.1 / 9.8 us.
-template <typename T>
-__global__ __launch_bounds__(256) void pct_attend_join_many_kernel(AttendParams p) {
-  const int lane = threadIdx.x & 63, h = lane >> 5, d = (lane & 31) * 4;
-  const int64_t rows = (int64_t)p.batch * p.kv_heads * p.rows, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= rows) return;
-  const int r = (int)(at % p.rows), bh = (int)(at / p.rows);
-  const bool none = allowed_keys(p, bh / p.kv_heads) == 0;
-  const float2 st = lane < p.splits ? p.part_stats[lane * rows + at] : make_float2(kLowest, 0.f);  // (64 splits at most)
-  const float ref = wave_max(st.x), f = __builtin_amdgcn_exp2f(st.x - ref), sum = wave_sum(f * st.y);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = 0; s < p.splits; s += 2) {
-    const float g = __shfl(f, s + h);
-    if (s + h < p.splits && d < p.dim) {
-      const float4 x = *(const float4*)(p.part + ((s + h) * rows + at) * p.dim + d);
-      o.x += g * x.x; o.y += g * x.y; o.z += g * x.z; o.w += g * x.w;
-    }
-  }
-  o.x += other_half(o.x); o.y += other_half(o.y); o.z += other_half(o.z); o.w += other_half(o.w);
-  const float inv = none ? 0.f : 1.f / sum;
-  if (lane == 0 && p.stats) p.stats[at] = none ? make_float2(0.f, INFINITY) : make_float2(ref, sum);
-  const Work w = {bh / p.kv_heads, bh % p.kv_heads, 0, 0};
-  if (h == 0 && d < p.dim) store4<T>((T*)p.out + out_head(p, w) + out_row(p, r) + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 // P of the backward pass: float32 keeps the forward's reference point and sum apart (their logarithm's rounding would be a
@@ -965,8 +939,7 @@ template <typename T> struct Attend {
       if (c.waves <= 2) launch<4 * Tile<T, DP, 32>::BYTES>(pct_attend_kernel<T, DP, W, 32>, g, c.waves, s, p);
       else launch<4 * Tile<T, DP>::BYTES>(pct_attend_kernel<T, DP, W, Type<T>::ROWS>, g, c.waves, s, p);
     });
-    if (c.splits > 8) pct_attend_join_many_kernel<T><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(p);
-    else if (c.splits > 1) pct_attend_join_kernel<T><<<(unsigned)((rows * (p.dim / 4) + 255) / 256), 256, 0, s>>>(p);
+    if (c.splits > 1) pct_attend_join_kernel<T><<<(unsigned)((rows * (p.dim / 4) + 255) / 256), 256, 0, s>>>(p);
     return policy_launched("attention kernel");
   }
   static int backward(AttendParams& p, char* ws, hipStream_t s) {
