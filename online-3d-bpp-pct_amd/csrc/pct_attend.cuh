@@ -845,7 +845,8 @@ __global__ __launch_bounds__(256) void pct_attend_sum_kernel(const float* part, 
 }
 
 // How the work is cut.  Resident rows: 32 to a wavefront, as many wavefronts to a workgroup as there are rows for (they share a
-// staged tile), but fewer while that leaves compute units without a workgroup.  Streamed rows: split over workgroups until
+// staged tile), 8 or at most 4 (5 to 7 load a compute unit's four SIMDs unevenly and leave no room for another workgroup: 90 heads x
+// 1300, D = 128, bfloat16, forward 150 us with 7, 112 with 4), and fewer while that leaves compute units without a workgroup.  Streamed rows: split over workgroups until
 // about eight wavefronts per compute unit are there, in parts of at least four tiles (64 x 50 x 131, float32: 5 tiles in two parts
 // 12.2 + 4.0 us for the join, in one 14); the partial results are joined after.
 struct Cut { int waves, tiles, splits; };
@@ -853,6 +854,10 @@ inline Cut cut(int64_t resident, int64_t streamed_tiles, int64_t heads, int max_
   const int64_t t = (resident + 31) / 32;
   int64_t w = t < max_waves ? t : max_waves, blocks = (t + w - 1) / w;
   w = (t + blocks - 1) / blocks;
+  if (w > 4 && w < 8) {
+    w = 4;
+    blocks = (t + w - 1) / w;
+  }
   while (heads * blocks < 256 && w > 1) {
     w = (w + 1) / 2;
     blocks = (t + w - 1) / w;
@@ -863,7 +868,7 @@ inline Cut cut(int64_t resident, int64_t streamed_tiles, int64_t heads, int max_
   return Cut{(int)w, (int)blocks, (int)s};
 }
 
-// wavefronts to a workgroup: 8, two to a SIMD, where a wavefront's registers allow it (256 each)
+// the wavefronts to a workgroup that a kernel is compiled for: 8, two to a SIMD, where a wavefront's registers allow it (256 each)
 template <typename T, int DP> constexpr int max_waves() { return sizeof(T) == 4 && DP > 64 ? 4 : 8; }
 
 // a launch with the LDS of four tiles, which may be more than the runtime's default limit of 64 KiB
@@ -881,19 +886,29 @@ template <typename T> struct Attend {
     if (dim <= 96) return f(std::integral_constant<int, 96>());
     return f(std::integral_constant<int, 128>());
   }
-  // Of few wavefronts to a head, small workgroups make better use of the chip: they wait for each other less, and where a part
-  // of unknown size of a short masked row is allowed, those behind it end at once.  Measured (4096 x 131 x 131, float32, a third
-  // of the keys allowed / 2048 x 4 heads x 200 x 401, bfloat16), with up to 8, 4, 2 wavefronts: forward 224, 168, 192 / 138, 128,
-  // 145 us; dq 342, 315, 263 / 215, 202, 227; dk and dv 481, 612, 305 / 460, 481, 305.  Of many (4 x 16 heads x 2048 x 4096) 8
-  // are the best by 5 to 10 %.
+  // Wavefronts to a workgroup: 4, from which two or three workgroups fit a compute unit and wait for each other's products.  Times below
+  // are us with up to 2 / 4 / 8, over 131 to 5000 rows, every type and four head sizes; fewer than 256 workgroups are cut further (cut).
+  //  * forward, 16-bit, 1024 rows and more: 8 read a tile half as often.  64 heads x 2048 x 2048: D = 32 158 / 123 / 115, 64 234 / 183 /
+  //    170, 128 461 / 328 / 306, but 96 336 / 253 / 282 (its registers).  Below 1024 rows they gain nothing (512: 132 / 97 / 100).
+  //  * dq, dk and dv, 16-bit, D = 128, 1024 rows and more, all keys allowed: of the whole backward pass 4 x 16 heads x 2048 x 4096
+  //    1528 / 1099 / 1083 by dq's, 1793 / 1145 / 1100 by dk's and dv's; with a mask 4 (64 heads x 2048: 1183 / 818 / 930).
+  //  * dq of float32, up to 512 rows: 2, since few rows to a head leave the last workgroup half empty -- 4096 x 131 x 131, D = 64 531 /
+  //    605 / 641, 200 rows 662 / 660 / 685, 450 rows 1325 / 1294 / 1346.
+  //  * dk and dv of float32, up to 512 keys of which not all are allowed: 2, whose workgroups end at once behind the allowed ones --
+  //    4096 x 131 530 / 601 / 741, 512 x 450 1326 / 1357 / 1466; 16-bit 2048 x 4 x 401, D = 32 414 / 389 / 428, 512 x 450, D = 128 741 /
+  //    559 / 600, so 4 there.
   static Cut cut_q(const AttendParams& p, bool dq) {
-    int mw = by_dim(p.dim, [](auto d) { return max_waves<T, d.value>(); });
-    if (p.rows <= 512) mw = dq && sizeof(T) == 4 ? 2 : 4;
+    const bool all = !p.list && !p.lengths;
+    int mw = 4;
+    if (sizeof(T) == 2 && p.rows >= 1024 && (dq ? all && p.dim > 96 : p.dim <= 64 || p.dim > 96)) mw = 8;
+    if (sizeof(T) == 4 && dq && p.rows <= 512) mw = 2;
     return cut(p.rows, (p.k_len + Type<T>::ROWS - 1) / Type<T>::ROWS, (int64_t)p.batch * p.kv_heads, mw);
   }
   static Cut cut_k(const AttendParams& p) {
-    int mw = by_dim(p.dim, [](auto d) { return max_waves<T, d.value>(); });
-    if (p.k_len <= 512) mw = p.list || p.lengths ? 2 : 4;
+    const bool all = !p.list && !p.lengths;
+    int mw = 4;
+    if (sizeof(T) == 2 && all && p.dim > 96 && p.k_len >= 1024) mw = 8;
+    if (sizeof(T) == 4 && !all && p.k_len <= 512) mw = 2;
     return cut(p.k_len, (p.rows + Type<T>::ROWS - 1) / Type<T>::ROWS, (int64_t)p.batch * p.kv_heads, mw);
   }
   // the partial statistics, up to where the partial results start (those are read 16 bytes at a time)
