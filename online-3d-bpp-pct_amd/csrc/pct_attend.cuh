@@ -310,7 +310,7 @@ struct Power {
 // Measured: 4 x 16 heads x 2048 x 4096 x 128 bfloat16 331 us, 830 TFLOP/s (a library product of 8192^3: 1134) -- two wavefronts to a
 // SIMD that wait for their own products and exponentials in turn; 2048 x 4 x 200 x 401 x 32 with 29 % of the keys 128 us, where
 // vector instructions are 59 % busy and HBM moves 2.6 TB/s; 4096 x 131 x 131 x 64 float32 163 us, its matrix instructions at 35 % of
-// their peak; single queries, 16 x 8 heads x 16384 x 128, 161 us, 5 TB/s.
+// their peak; single queries, 16 x 8 heads x 16384 x 128, 156 us, 5.2 TB/s.
 template <typename T, int DP, int MAXW, int R>
 __global__ __launch_bounds__(64 * MAXW) void pct_attend_kernel(AttendParams p) {
   using L = Tile<T, DP, R>;
@@ -663,7 +663,7 @@ __global__ __launch_bounds__(64 * MAXW) void pct_attend_dq_kernel(AttendParams p
 // --------------------------------------------------------------------------------------------------------------- dk, dv
 // The same tiles with the sides changed: keys stay, q and d_out pass.  S and dP are computed a second time, which costs two products
 // of seven and needs neither atomics nor dS in memory.  Measured: 4 x 16 x 2048 x 4096 x 128 bfloat16 611 us, 900 TFLOP/s over four
-// products; 2048 x 4 x 200 x 401 x 32 174 us; 4096 x 131 x 131 x 64 float32 250 us, 46 % of the matrix peak.
+// products; 2048 x 4 x 200 x 401 x 32 160 us; 4096 x 131 x 131 x 64 float32 250 us, 46 % of the matrix peak.
 template <typename T, int DP, int MAXW>
 __global__ __launch_bounds__(64 * MAXW) void pct_attend_dkv_kernel(AttendParams p) {
   using L = Tile<T, DP>;

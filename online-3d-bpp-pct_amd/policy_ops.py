@@ -399,6 +399,8 @@ def cross_attention(q, k, v, key_mask=None, key_lengths=None, scale=None):
     Lk, and Lq * H / Hk, are below 2^29, and a call is refused whose launch would hold more than 2^32 threads (some 2^26
     heads times groups of 32 rows).  The mask and the lengths may be written over once the call has returned, in its stream's
     order: the backward pass reads what was made of them.
+    Scores, sums and statistics are float32; in 16-bit types the weights and the scores' gradients are rounded to the type before they
+    are multiplied with v, k, q and the output's gradient, as the results are.
     `scale` is positive, 1 / sqrt(D) if not given.  q, k, v and the output's gradient are read where they are if their rows
     are contiguous and start on 16 bytes, else from a copy."""
     name = "cross_attention"
