@@ -75,3 +75,14 @@ def test_infinite_values_and_gradients_stay_in_their_columns(lq, lk, dtype):
         keep = [i for i in range(d) if i != 7]
         assert (got[1, :, 0, 7] == -math.inf).all(), at
         assert torch.equal(got[0], want[0]) and torch.equal(got[1][..., keep], want[1][..., keep]), at
+
+
+# 8 wavefronts to a workgroup in the forward, in dq, in dk and dv; lengths that would make 5 to 7, and just not 8
+CUTS = [(16, 1024, 70, 4, 4, 64), (64, 1024, 70, 1, 1, 128), (64, 40, 1024, 1, 1, 128), (64, 1100, 35, 1, 1, 64), (64, 1023, 9, 2, 1, 104), (32, 130, 1300, 2, 2, 120)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", CUTS, ids=str)
+def test_long_rows_and_keys_of_many_heads(shape, dtype):
+    _check(shape, dtype, "none", 44)
+    _check(shape, dtype, "lengths", 45)
